@@ -410,6 +410,135 @@ int qr_decoder_forward(qr_decoder* dec, int token, int pos, float* logits, float
 int qr_decoder_prefill(qr_decoder* dec, const int32_t* tokens, int n, int pos0, int chunk,
                        float* logits, float* x_out, int flags);
 
+/* ---- a KV pool that sequences share ---------------------------------------- */
+
+/* Pages of 8-bit K and V that several sequences share: batches, beams, the
+ * continuations of one prompt, speculative verification.  No counterpart in
+ * the reference, whose cache holds one sequence; the calls below promise the
+ * formulas they state in fp32 accuracy, not another build's bits.
+ *
+ * All memory is the caller's, on the context's device:
+ *   data   int8 [n_layers][n_pages][n_kv_heads][page / 16][2][16 * head_dim],
+ *          16-byte aligned: a block of 16 tokens of one kv head as its K rows
+ *          [16][head_dim], then its V columns [head_dim][16];
+ *   scale  fp32 [n_layers][n_pages][n_kv_heads][page / 16][2], 8-byte aligned: the
+ *          block's K and V scales (a cached value is its int8 times the scale);
+ *   table  int32 [n_seqs][max_pages]: the page of each page's worth of tokens
+ *          of a sequence, -1 behind them;
+ *   len    int32 [n_seqs]: the tokens of each sequence;
+ *   refs   int32 [n_pages]: the table entries that name a page (0: free).
+ * page is a power of two from 16 to 65536, head_dim a multiple of 32 up to 256,
+ * n_kv_heads up to 1024.
+ * Every call reads and writes them on the context's stream and waits for
+ * nothing, so all of them can be captured into a graph (after one run that
+ * grew the context's scratch).
+ *
+ * A list argument (seqs, dst, ...) is a device array of n entries, n <=
+ * QR_KV_MAX_LIST.  What a list asks for is checked on the device: `status`
+ * (device int32, optional) receives QR_OK; QR_ERR_INVALID for a sequence that
+ * does not exist, one listed twice (extend, and dst of assign), a negative
+ * number, or more tokens than max_pages hold; QR_ERR_NOMEM where the free pages do not
+ * suffice.  A call whose status is not QR_OK has changed nothing. */
+#define QR_KV_BLOCK 16
+#define QR_KV_MAX_LIST 4096
+#define QR_KV_MAX_SEQS 65536
+#define QR_KV_MAX_ROWS (1 << 22)
+typedef struct {
+    int n_layers;
+    int n_pages;
+    int page;
+    int n_kv_heads;
+    int head_dim;
+    int n_seqs;
+    int max_pages;
+    int8_t* data;
+    float* scale;
+    int32_t* table;
+    int32_t* len;
+    int32_t* refs;
+} qr_kv_pool;
+
+/* No page in use: table all -1, len and refs all 0. */
+int qr_kv_pool_reset(qr_ctx* ctx, const qr_kv_pool* pool);
+
+/* Sequence seqs[i] grows by add[i] tokens: it takes the pages that they need,
+ * the free pages in ascending order in the order of the list.  Where its last
+ * page is partly filled and shared, it first takes a copy of it (of all
+ * layers): in the order of the list, each of them but the last that holds it. */
+int qr_kv_pool_extend(qr_ctx* ctx, const qr_kv_pool* pool, const int32_t* seqs,
+                      const int32_t* add, int n, int32_t* status);
+
+/* Sequence dst[i] becomes what src[i] was when the call began: its pages are
+ * shared, none is copied, and what dst[i] held is given back.  A fork (dst
+ * empty), a beam's reordering (dst and src of the same sequences). */
+int qr_kv_pool_assign(qr_ctx* ctx, const qr_kv_pool* pool, const int32_t* dst,
+                      const int32_t* src, int n, int32_t* status);
+
+/* Sequence seqs[i] keeps its first keep[i] tokens (all of them where it has no
+ * more; 0 frees it) and gives back the pages behind them.  A sequence listed
+ * twice keeps the smaller number. */
+int qr_kv_pool_trim(qr_ctx* ctx, const qr_kv_pool* pool, const int32_t* seqs,
+                    const int32_t* keep, int n, int32_t* status);
+
+/* The pages in use move to the lowest numbers: with L of them, those numbered L
+ * or more go, in ascending order, to the free pages below L.  Tables and refs
+ * follow.  n_live (device int32, optional) receives L, map (device int32
+ * [n_pages], optional) each page's new number, -1 for a free page. */
+int qr_kv_pool_compact(qr_ctx* ctx, const qr_kv_pool* pool, int32_t* map, int32_t* n_live);
+
+/* The rows of a ragged batch: T rows (at most QR_KV_MAX_ROWS), of which start[i] .. start[i + 1] - 1
+ * (start: device int32 [n + 1], ascending) are sequence seqs[i]'s (seqs null:
+ * sequence i's), n up to QR_KV_MAX_SEQS; they stand for its last positions, so a call that brings new
+ * tokens extends first.  Rows that no sequence owns are left as they are.
+ *
+ * store quantizes K and V rows (fp32, head h's values at h * head_dim, row
+ * stride kv_stride, a multiple of 4, 16-byte aligned) into layer `layer`.  A block's scale becomes
+ * max(its scale if it holds older tokens, max |x| / 127) over the new finite
+ * values; new values are x / scale rounded to the nearest even integer, and
+ * where the scale grew older ones are rounded to the new one.  NaN is stored as 0,
+ * an infinity as +-127.  A row before position 0, or where the table has no
+ * page, is not stored.  No sequence may be listed twice, and none of the pages
+ * written shared: extend sees to that.
+ * load reads rows back as fp32 (zeros for a row before position 0 or without a page). */
+int qr_kv_pool_store(qr_ctx* ctx, const qr_kv_pool* pool, int layer, const int32_t* seqs,
+                     const int32_t* start, int n, int T, const float* k, const float* v,
+                     long kv_stride);
+int qr_kv_pool_load(qr_ctx* ctx, const qr_kv_pool* pool, int layer, const int32_t* seqs,
+                    const int32_t* start, int n, int T, float* k, float* v, long kv_stride);
+
+/* Attention of the batch's query rows over their sequences' cached tokens:
+ * out[r][h] = sum_t w_t v_t / sum_t w_t with w_t = exp(scale * q[r][h] . k_t),
+ * over the positions t up to the row's own, and of those the last `window` (0:
+ * all).  Query head h reads kv head h / (n_heads / n_kv_heads).  q and out are
+ * fp32 rows of n_heads * head_dim values, strides multiples of 4, 16-byte
+ * aligned.  scale <= 0 means 1 / sqrtf(head_dim).  max_len bounds the
+ * sequences' lengths for the split of the work (0: max_pages * page); longer
+ * sequences are served all the same.  A row that sees no token (one before
+ * position 0) gives zeros, a q row that is not finite NaN. */
+int qr_kv_pool_attention(qr_ctx* ctx, const qr_kv_pool* pool, int layer, const int32_t* seqs,
+                         const int32_t* start, int n, int T, int n_heads, const float* q,
+                         long q_stride, float* out, long out_stride, int max_len, int window,
+                         float scale);
+
+/* ---- log probabilities ------------------------------------------------------ */
+
+/* For each of `rows` rows of `vocab` logits (row stride `stride`), with p =
+ * softmax(row): lp[r] = log p[targets[r]]; entropy[r] = -sum p log p; rank[r]
+ * = the number of logits ahead of the target's (greater ones, and equal ones
+ * of lower index); top_id / top_lp [r][n_top], n_top <= QR_LOGPROBS_MAX_TOP: the most
+ * probable tokens, equal ones by ascending index, with their log
+ * probabilities (id -1 and -inf behind the vocabulary).  Each output may be
+ * null; targets may be null where lp and rank are.  A target outside the
+ * vocabulary gives lp 0 and rank -1.  Logits of -inf have probability 0; a row
+ * of nothing else gives lp -inf, entropy 0.  A row that holds a NaN or +inf
+ * gives NaN for lp, entropy and top_lp; in its order a NaN counts as -inf.  Beside
+ * qr_decoder_prefill with QR_PREFILL_ALL_LOGITS it scores a prompt; no
+ * counterpart in the reference. */
+#define QR_LOGPROBS_MAX_TOP 64
+int qr_logprobs(qr_ctx* ctx, const float* logits, long stride, int rows, int vocab,
+                const int32_t* targets, float* lp, float* entropy, int32_t* rank, int n_top,
+                int32_t* top_id, float* top_lp);
+
 /* ---- GGUF files (src/gguf.c, src/model.c:253-449) ----------------------- */
 
 /* A parsed GGUF container.  qr_gguf_parse reads a buffer the caller keeps

@@ -21,6 +21,9 @@ int set_error(int code, const char* fmt, ...);
 hipStream_t ctx_stream(qr_ctx* c);
 int ctx_device(qr_ctx* c);
 bool ctx_capturing(qr_ctx* c);
+// At least `need` bytes of the context's scratch (the calls on a context are
+// ordered by its stream and share it); refused under capture where it would grow.
+int ctx_scratch_get(qr_ctx* c, size_t need, const char* who, void** out);
 int moe_check(const qr_moe_layer* L, const char* who);
 int gemv_check(uint32_t type, int order, const void* w, int n, int d, const char* who);
 

@@ -1,0 +1,103 @@
+// qr_kv_pool.h -- the layout of a shared 8-bit KV pool (qr_kv_pool of
+// qr_hip.h) as its kernels see it, and how a ragged batch's rows are found.
+//
+// A block is 16 tokens of one kv head of one layer: int8 K [16][hd], then int8
+// V [hd][16], and two fp32 scales.  V lies column by column, so that 16 bytes
+// of it are one column's 16 tokens: what a lane of a 16x16x64 int8 MFMA takes
+// as its operand of the value product.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "qr_internal.h"
+
+namespace qr {
+
+constexpr int kKvBlock = 16;  // tokens of a scale
+
+// One layer of a pool.
+struct PoolView {
+  int8_t* data;
+  float* scale;
+  const int32_t* table;
+  const int32_t* len;
+  int n_pages, n_kv_heads, hd, n_seqs, max_pages;
+  int page_shift;
+};
+
+// The rows of a ragged batch: sequence i owns rows start[i] .. start[i + 1] - 1,
+// which stand for its last positions.  T rows exist; values outside 0 .. T are
+// cut to it, so a bad array reads and writes no row that is not there.
+struct Ragged {
+  const int32_t* seqs;   // [n] rows of the table, or null: 0 .. n - 1
+  const int32_t* start;  // [n + 1]
+  int n, T;
+};
+
+__device__ inline int ragged_start(const Ragged& r, int i) {
+  const int s = r.start[i];
+  return s < 0 ? 0 : s > r.T ? r.T : s;
+}
+
+// Sequence i's row of the table, its rows and its length (0 where the row of
+// the table does not exist).
+struct SeqRows {
+  int seq, row0, m, len;
+};
+__device__ inline SeqRows seq_rows(const PoolView& p, const Ragged& r, int i) {
+  SeqRows s;
+  s.row0 = ragged_start(r, i);
+  s.m = ragged_start(r, i + 1) - s.row0;
+  if (s.m < 0) s.m = 0;
+  s.seq = r.seqs ? r.seqs[i] : i;
+  if ((unsigned)s.seq >= (unsigned)p.n_seqs) {
+    s.seq = 0;
+    s.len = 0;
+    return s;
+  }
+  const long cap = (long)p.max_pages << p.page_shift;
+  const int n = p.len[s.seq];
+  s.len = n < 0 ? 0 : n > cap ? (int)cap : n;
+  return s;
+}
+
+// Which sequence a slot serves, where each sequence's rows are cut into pieces
+// of q rows: sequence i has the slots from start[i] / q + extra * i on.  There
+// are never fewer than its pieces (floor(b / q) - floor(a / q) + 1 >=
+// ceil((b - a) / q)), so the host sizes the grid by T / q + extra * n without
+// knowing the lengths, and a slot without a piece ends.  Returns the sequence
+// and sets *piece.
+__device__ inline int slot_seq(const Ragged& r, int slot, int q, int extra, int* piece) {
+  int lo = 0, hi = r.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (ragged_start(r, mid) / q + extra * mid <= slot)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  *piece = slot - (ragged_start(r, lo) / q + extra * lo);
+  return lo;
+}
+
+// The physical page of a sequence's logical page, -1 where there is none.
+__device__ inline int page_at(const PoolView& p, int seq, int lp) {
+  if ((unsigned)lp >= (unsigned)p.max_pages) return -1;
+  const int g = p.table[(size_t)seq * p.max_pages + lp];
+  return (unsigned)g < (unsigned)p.n_pages ? g : -1;
+}
+
+// Index of a block of the layer: (page, kv head, block of the page).
+__device__ inline size_t block_at(const PoolView& p, int page, int kvh, int b) {
+  return (((size_t)page * p.n_kv_heads + kvh) << (p.page_shift - 4)) + (size_t)b;
+}
+
+// qr_kv_attn.hip
+hipError_t kv_attention_launch(const PoolView& p, const Ragged& r, int n_heads, const float* q,
+                               long q_stride, float* out, long out_stride, int max_len, int window,
+                               float scale, void* work, hipStream_t st);
+size_t kv_attention_scratch(const PoolView& p, const Ragged& r, int n_heads, int max_len,
+                            int window);
+
+}  // namespace qr

@@ -243,6 +243,9 @@ int set_error(int code, const char* fmt, ...) {
 hipStream_t ctx_stream(qr_ctx* c) { return c->stream; }
 int ctx_device(qr_ctx* c) { return c->device; }
 bool ctx_capturing(qr_ctx* c) { return capturing(c); }
+int ctx_scratch_get(qr_ctx* c, size_t need, const char* who, void** out) {
+  return ctx_scratch(c, need, who, out);
+}
 }  // namespace qr
 
 extern "C" {

@@ -60,6 +60,19 @@ class Model(C.Structure):
     ]
 
 
+class KvPool(C.Structure):
+    """qr_kv_pool (include/qr_hip.h): a KV pool that sequences share; pointers
+    are device addresses of memory that the caller keeps."""
+    _fields_ = [
+        ("n_layers", C.c_int), ("n_pages", C.c_int), ("page", C.c_int), ("n_kv_heads", C.c_int),
+        ("head_dim", C.c_int), ("n_seqs", C.c_int), ("max_pages", C.c_int),
+        ("data", _vp), ("scale", _vp), ("table", _vp), ("len", _vp), ("refs", _vp),
+    ]
+
+
+KV_BLOCK, KV_MAX_LIST, KV_MAX_SEQS, KV_MAX_ROWS = 16, 4096, 65536, 1 << 22
+LOGPROBS_MAX_TOP = 64
+
 KV_F32, KV_F16, KV_Q8_0 = 0, 1, 2
 MOE_PATH_AUTO, MOE_PATH_GEMV, MOE_PATH_MFMA = 0, 1, 2
 DEC_GRAPH = 1
@@ -130,6 +143,20 @@ _SIGS = {
     "qr_decoder_forward": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp]),
     "qr_decoder_prefill": (C.c_int, [_vp, C.POINTER(C.c_int32), C.c_int, C.c_int, C.c_int, _vp, _vp,
                                      C.c_int]),
+    "qr_kv_pool_reset": (C.c_int, [_vp, C.POINTER(KvPool)]),
+    "qr_kv_pool_extend": (C.c_int, [_vp, C.POINTER(KvPool), _vp, _vp, C.c_int, _vp]),
+    "qr_kv_pool_assign": (C.c_int, [_vp, C.POINTER(KvPool), _vp, _vp, C.c_int, _vp]),
+    "qr_kv_pool_trim": (C.c_int, [_vp, C.POINTER(KvPool), _vp, _vp, C.c_int, _vp]),
+    "qr_kv_pool_compact": (C.c_int, [_vp, C.POINTER(KvPool), _vp, _vp]),
+    "qr_kv_pool_store": (C.c_int, [_vp, C.POINTER(KvPool), C.c_int, _vp, _vp, C.c_int, C.c_int,
+                                   _vp, _vp, C.c_long]),
+    "qr_kv_pool_load": (C.c_int, [_vp, C.POINTER(KvPool), C.c_int, _vp, _vp, C.c_int, C.c_int,
+                                  _vp, _vp, C.c_long]),
+    "qr_kv_pool_attention": (C.c_int, [_vp, C.POINTER(KvPool), C.c_int, _vp, _vp, C.c_int,
+                                       C.c_int, C.c_int, _vp, C.c_long, _vp, C.c_long, C.c_int,
+                                       C.c_int, C.c_float]),
+    "qr_logprobs": (C.c_int, [_vp, _vp, C.c_long, C.c_int, C.c_int, _vp, _vp, _vp, _vp, C.c_int,
+                              _vp, _vp]),
     "qr_gguf_parse": (C.c_int, [_vp, C.c_size_t, C.POINTER(_vp)]),
     "qr_gguf_open": (C.c_int, [C.c_char_p, C.POINTER(_vp)]),
     "qr_gguf_close": (C.c_int, [_vp]),
@@ -232,6 +259,11 @@ class Device:
         if self.ctx is not None:
             self.lib.qr_ctx_destroy(_vp(self.ctx))
             self.ctx = None
+
+    def set_stream(self, stream):
+        """qr_ctx_set_stream: the calls go to this hipStream_t (an int; 0 or None:
+        the context's own stream)."""
+        self._check(self.lib.qr_ctx_set_stream(self.ctx, _vp(stream or None)), "qr_ctx_set_stream")
 
     def set_moe_path(self, path):
         """QR_MOE_PATH_*: 0 auto, 1 grouped GEMV, 2 int8 MFMA (T > 1)."""
@@ -372,6 +404,61 @@ class Device:
         self._check(self.lib.qr_attention(self.ctx, _vp(q_ptr), _vp(kc_ptr), _vp(vc_ptr),
                                           _vp(ptab_ptr), page, kv_type, npos, n_heads, n_kv_heads,
                                           head_dim, _vp(att_ptr), _vp(out_ptr)), "qr_attention")
+
+    # ---- a KV pool that sequences share (pool: KvPool; pointers are device addresses)
+    def kv_pool_reset(self, pool):
+        self._check(self.lib.qr_kv_pool_reset(self.ctx, pool), "qr_kv_pool_reset")
+
+    def kv_pool_extend(self, pool, seqs_ptr, add_ptr, n, status_ptr=None):
+        """Sequence seqs[i] grows by add[i] tokens; status: device int32."""
+        self._check(self.lib.qr_kv_pool_extend(self.ctx, pool, seqs_ptr, add_ptr, n, status_ptr),
+                    "qr_kv_pool_extend")
+
+    def kv_pool_assign(self, pool, dst_ptr, src_ptr, n, status_ptr=None):
+        """Sequence dst[i] becomes what src[i] was, sharing its pages."""
+        self._check(self.lib.qr_kv_pool_assign(self.ctx, pool, dst_ptr, src_ptr, n, status_ptr),
+                    "qr_kv_pool_assign")
+
+    def kv_pool_trim(self, pool, seqs_ptr, keep_ptr, n, status_ptr=None):
+        """Sequence seqs[i] keeps its first keep[i] tokens (0 frees it)."""
+        self._check(self.lib.qr_kv_pool_trim(self.ctx, pool, seqs_ptr, keep_ptr, n, status_ptr),
+                    "qr_kv_pool_trim")
+
+    def kv_pool_compact(self, pool, map_ptr=None, live_ptr=None):
+        """The pages in use move to the lowest numbers."""
+        self._check(self.lib.qr_kv_pool_compact(self.ctx, pool, map_ptr, live_ptr),
+                    "qr_kv_pool_compact")
+
+    def kv_pool_store(self, pool, layer, seqs_ptr, start_ptr, n, T, k_ptr, v_ptr, stride=None):
+        """Quantize T rows, start[i] .. start[i + 1] - 1 of sequence seqs[i], into
+        its last positions (seqs_ptr None: sequence i)."""
+        self._check(self.lib.qr_kv_pool_store(
+            self.ctx, pool, layer, seqs_ptr, start_ptr, n, T, k_ptr, v_ptr,
+            pool.n_kv_heads * pool.head_dim if stride is None else stride), "qr_kv_pool_store")
+
+    def kv_pool_load(self, pool, layer, seqs_ptr, start_ptr, n, T, k_ptr, v_ptr, stride=None):
+        """The rows of the last positions read back as fp32."""
+        self._check(self.lib.qr_kv_pool_load(
+            self.ctx, pool, layer, seqs_ptr, start_ptr, n, T, k_ptr, v_ptr,
+            pool.n_kv_heads * pool.head_dim if stride is None else stride), "qr_kv_pool_load")
+
+    def kv_pool_attention(self, pool, layer, seqs_ptr, start_ptr, n, T, n_heads, q_ptr, out_ptr,
+                          max_len=0, window=0, scale=0.0, q_stride=None, out_stride=None):
+        """Attention of T query rows over their sequences' cached tokens."""
+        row = n_heads * pool.head_dim
+        self._check(self.lib.qr_kv_pool_attention(
+            self.ctx, pool, layer, seqs_ptr, start_ptr, n, T, n_heads, q_ptr,
+            row if q_stride is None else q_stride, out_ptr,
+            row if out_stride is None else out_stride, max_len, window, scale),
+            "qr_kv_pool_attention")
+
+    def logprobs(self, logits_ptr, rows, vocab, targets_ptr, lp_ptr, entropy_ptr, rank_ptr, n_top=0,
+                 top_id_ptr=None, top_lp_ptr=None, stride=None):
+        """Log probability and rank of a token of each row, the entropy, and the
+        n_top most probable tokens; any output may be None."""
+        self._check(self.lib.qr_logprobs(self.ctx, logits_ptr, vocab if stride is None else stride,
+                                         rows, vocab, targets_ptr, lp_ptr, entropy_ptr, rank_ptr,
+                                         n_top, top_id_ptr, top_lp_ptr), "qr_logprobs")
 
 
 class Decoder:
