@@ -13,15 +13,19 @@
 // v_mfma_i32_16x16x64_i8 at twice the rate of bf16 and read the cache's bytes
 // as they lie, so nothing is dequantized on the way.
 //
-// A wave serves 16 rows (queries times the query heads of a kv head) and takes
-// 64 tokens a step.  Its four lane groups g = lane / 16 own a block each:
+// A workgroup of four waves serves a tile of 16 or 32 rows (queries times the query
+// heads of a kv head) and takes 256 tokens a round, a wave 64 of them.  A wave's four
+// lane groups g = lane / 16 own a block each:
 //   scores: A = 16 tokens of K in four tiles, tile t's row 4 g + i being token
 //   16 g + 4 t + i; B = the rows' digits.  D then leaves row lane % 16 the four
 //   tokens 4 t .. 4 t + 3 of block g, over the four tiles all 16 of them.
 //   values: A = 16 columns of V, whose 16 bytes are a block's 16 tokens of a
 //   column; B = the digits of the weights, in the lanes and bytes where the scores
-//   left them.  No value crosses a lane between the two products, and the scales
-//   of a block are one pair of numbers per lane.
+//   left them, so no weight crosses a lane.
+// The values' columns are what the waves share out: each reads all four waves'
+// digits from LDS (12 KiB) and sums 256 tokens in integers before anything is
+// rounded.  A wave that kept all columns of its own tokens instead converted four
+// times as many sums, held 206 registers for 142, and ended in a join of the waves.
 //
 // The weights carry V's scale: with vs = f 2^e (1 <= f < 2), w_t = f 2^(s_t
 // log2(e) + e - M) against the running maximum M of the exponents, so the
@@ -36,9 +40,10 @@ namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 
-constexpr int kRows = 16;   // rows of a tile
 constexpr int kStep = 64;   // tokens of a wave's step
-constexpr int kWaves = 4;   // of a workgroup, taking the steps of its tokens in turn
+constexpr int kWaves = 4;   // of a workgroup
+constexpr int kRound = kStep * kWaves;
+constexpr int kMaxParts = 1024;  // of a tile's tokens
 constexpr float kNone = -INFINITY;
 // Weights below 2 become whole numbers below 2^23 - 0x8080: added to 2^23 +
 // 0x8080 they are the low mantissa bits of a float, and its three low bytes the
@@ -66,12 +71,12 @@ struct AttnArgs {
   long q_stride, out_stride;
   int n_heads, group;   // query heads, query heads per kv head
   int hgroups, hpt;     // groups of at most 16 of a kv head's query heads, heads of each
-  int qpt;              // queries of a tile
+  int rt, qpt, extra;   // 16-row sets of a tile, queries of it, slots beyond T / qpt for each sequence
   int slots, splits;    // tiles of a head group, parts that a tile's tokens are cut into
   int chunk;            // tokens of a part, a multiple of kStep
   int window;
   float scale2;         // scale * log2(e)
-  float* part;          // [tile, head][splits][kRows][hd], then [..][kRows][2]
+  float* part;          // [tile, head][splits][row][hd], then [..][row][2]
   float* ml;
 };
 
@@ -79,8 +84,7 @@ __device__ inline Tile tile_of(const AttnArgs& a, int slot) {
   Tile t;
   t.queries = 0;
   int piece;
-  const int i = slot_seq(a.r, slot, a.qpt, 1, &piece);
-  const SeqRows s = seq_rows(a.p, a.r, i);
+  const SeqRows s = slot_rows(a.p, a.r, slot, a.qpt, a.extra, &piece);
   const int at = piece * a.qpt;
   if (piece < 0 || at >= s.m) return t;
   t.row0 = s.row0 + at;
@@ -89,6 +93,18 @@ __device__ inline Tile tile_of(const AttnArgs& a, int slot) {
   t.len = s.len;
   t.pos0 = s.len - s.m + at;
   return t;
+}
+
+// Which tile and part a workgroup takes.  The last tiles, whose rows see most, come
+// first.  Workgroups go round the 8 XCDs in order, and a sequence's later parts are
+// empty where it is short, so neither the part nor the sequence may go with the
+// XCD: part after part, the tiles of each turned by some (32 sequences of up to 4096
+// tokens: 24.6 us, 35 with the eight parts of a tile side by side, every first part on one XCD).
+__device__ inline void work_of(const AttnArgs& a, int* slot, int* z) {
+  *z = (int)(blockIdx.x / a.slots);
+  int s = (int)(blockIdx.x % a.slots);
+  if (a.splits > 1) s = (s + *z + (*z >> 2) + (int)blockIdx.y) % a.slots;
+  *slot = a.slots - 1 - s;
 }
 
 // Tokens [*lo, *hi) that any row of the tile sees, *lo down to a step.
@@ -145,21 +161,26 @@ __device__ inline float rows_sum(float v) {
 __device__ inline int4 load16(const int8_t* p) { return *reinterpret_cast<const int4*>(p); }
 __device__ inline v4i as_v4(int4 x) { return v4i{x.x, x.y, x.z, x.w}; }
 
-// out = sum over the parts of w_s O_s / L, in O_s' own maximum: the joining of
-// two sums (m, l, o) and (m2, l2, o2).
+// The factor that takes a sum against maximum m to one against `to`.
 __device__ inline float lift(float m, float to) {
   return m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
 }
 
-template <int HD>
-__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pool_attn(AttnArgs a) {
-  constexpr int NC = (HD + 63) / 64;  // 64-column chunks of a K row
-  constexpr int NV = HD / 16;         // 16-column tiles of V
-  __shared__ float so[2][kRows][HD + 4];
-  __shared__ float sm[2][kRows][2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <int HD, int RT>
+__global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) void k_pool_attn(AttnArgs a) {
+  constexpr int NC = (HD + 63) / 64;            // 64-column chunks of a K row
+  constexpr int NV = (HD / 16 + 3) / kWaves;    // 16-column tiles of V for a wave
+  __shared__ int4 sp[kWaves][RT][3][64];        // the weights' digits
+  __shared__ int8_t sq[3][16 * RT][NC * 64 + 16];  // the rows' digits
+  __shared__ float sqs[16 * RT];                   // and what one of the last place stands for
+  __shared__ float smax[kWaves][RT][16];
+  __shared__ float ssum[kWaves][RT][16];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int slot = blockIdx.x / a.splits, z = blockIdx.x % a.splits, hy = blockIdx.y;
+  int slot, z;
+  work_of(a, &slot, &z);
+  const int hy = blockIdx.y;
   const int kvh = hy / a.hgroups, hg = hy % a.hgroups;
   const Tile t = tile_of(a, slot);
   if (t.queries == 0) return;
@@ -168,251 +189,305 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_pool_attn(AttnArgs a
   part_range(a, lo, hi, z, &tb, &te);
   if (tb >= te && a.splits > 1) return;  // the joining launch skips it too
 
-  // this lane's row
-  const int qi = n / a.hpt, hh = hg * a.hpt + n % a.hpt;
-  const bool row_ok = qi < t.queries && qi < a.qpt && hh < a.group;
-  const long row = t.row0 + qi;
-  const int head = kvh * a.group + hh;
-  int row_hi = row_ok ? t.pos0 + qi + 1 : 0;
-  int row_lo = row_ok && a.window > 0 ? row_hi - a.window : 0;
-  // positions before 0 see nothing
-  if (row_hi < 0) row_hi = 0;
-
-  // q's digits: the lane holds columns 64 c + 16 g .. + 15 of its row
-  v4i q0[NC], q1[NC], q2[NC];
-  float qs;
-  {
-    float x[NC][16], amax = 0.0f;
-    bool fine = true;
-#pragma unroll
-    for (int c = 0; c < NC; c++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        float4 f = make_float4(0, 0, 0, 0);
-        if (row_ok && (HD % 64 == 0 || 64 * c + 16 * g < HD))
-          f = *reinterpret_cast<const float4*>(a.q + row * a.q_stride + (long)head * HD + 64 * c +
-                                               16 * g + 4 * j);
-        x[c][4 * j] = f.x;
-        x[c][4 * j + 1] = f.y;
-        x[c][4 * j + 2] = f.z;
-        x[c][4 * j + 3] = f.w;
-      }
-#pragma unroll
-    for (int c = 0; c < NC; c++)
-#pragma unroll
-      for (int j = 0; j < 16; j++) {
-        const float f = fabsf(x[c][j]);
-        fine = fine && f <= 3.402823466e+38f;
-        amax = fmaxf(amax, f);
-      }
-    amax = rows_max(amax);
-    const float bad = rows_max(fine ? 0.0f : 1.0f);
-    // below 2^-96 a row's scores are 0 beside any scale of K that fp32 values give
-    amax = fmaxf(amax, 1.2621774e-29f);
-    const float inv = kQMax / amax;
-    qs = bad > 0.0f ? NAN : amax / kQMax * a.scale2;
-#pragma unroll
-    for (int c = 0; c < NC; c++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        uint32_t u[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float f = fminf(fmaxf(x[c][4 * j + i] * inv, -kQMax), kQMax);
-          u[i] = (uint32_t)((int)rintf(f) + 0x8080);
-        }
-        int e0, e1, e2;
-        digits4(u[0], u[1], u[2], u[3], &e0, &e1, &e2);
-        q0[c][j] = e0;
-        q1[c][j] = e1;
-        q2[c][j] = e2;
-      }
-  }
-
-  float o[NV][4];
-#pragma unroll
-  for (int d = 0; d < NV; d++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[d][i] = 0.0f;
-  float M = kNone, L = 0.0f;
-
-  const int kb = n >> 2;  // the block of the lane's K rows
-  const int8_t* const data = a.p.data;
-  // The lane's blocks of a step: kp / vp pages of K's and V's, -1 where there is none.
-  auto pages = [&](int T0, int* kp, int* vp) {
-    *kp = T0 + 16 * kb < te ? page_at(a.p, t.seq, (T0 + 16 * kb) >> a.p.page_shift) : -1;
-    *vp = T0 + 16 * g < te ? page_at(a.p, t.seq, (T0 + 16 * g) >> a.p.page_shift) : -1;
+  // Pages of a round's 16 blocks, one in each lane group's lanes; -1: none.
+  auto pages = [&](int T0) {
+    const int tok = T0 + 16 * n;
+    return tok < te ? page_at(a.p, t.seq, tok >> a.p.page_shift) : -1;
   };
   const int pmask = (1 << (a.p.page_shift - 4)) - 1;
-  int4 kr[4][NC];
+  const int8_t* const data = a.p.data;
+  int pg = pages(tb), pg1 = -1;
+
+  // this lane's rows
+  long row[RT];
+  int head[RT], row_hi[RT], row_lo[RT];
+  bool row_ok[RT];
+#pragma unroll
+  for (int r = 0; r < RT; r++) {
+    const int at = 16 * r + n, qi = at / a.hpt, hh = hg * a.hpt + at % a.hpt;
+    row_ok[r] = qi < t.queries && hh < a.group;
+    // a lane without a row computes row 0 again and writes nothing
+    row[r] = t.row0 + (row_ok[r] ? qi : 0);
+    head[r] = kvh * a.group + (row_ok[r] ? hh : hg * a.hpt);
+    // positions before 0 see nothing
+    row_hi[r] = row_ok[r] && t.pos0 + qi >= 0 ? t.pos0 + qi + 1 : 0;
+    row_lo[r] = a.window > 0 ? row_hi[r] - a.window : 0;
+  }
+
+  // q: kPer lanes share a row, four columns each; a wave takes every fourth set of rows.
+  constexpr int kPer = NC == 1 ? 16 : NC == 2 ? 32 : 64, kSets = 64 / kPer;
+  constexpr int kTurns = 16 * RT / (kWaves * kSets);
+  const int qc = lane % kPer * 4;
+  float4 x[kTurns];
+#pragma unroll
+  for (int i = 0; i < kTurns; i++) {
+    const int at = (i * kWaves + wave) * kSets + lane / kPer;
+    const int qi = at / a.hpt, hh = hg * a.hpt + at % a.hpt;
+    x[i] = make_float4(0, 0, 0, 0);
+    if (qi < t.queries && hh < a.group && qc < HD)
+      x[i] = *reinterpret_cast<const float4*>(a.q + (t.row0 + qi) * a.q_stride +
+                                              (long)(kvh * a.group + hh) * HD + qc);
+  }
+
+  // K of the wave's step, its blocks' scales, and V's columns of the round
+  int4 kr[4][NC], vr[NV][kWaves];
   float2 sc;
-  auto load_k = [&](int T0, int kp, int vp) {
-    const size_t bk = kp < 0 ? 0 : block_at(a.p, kp, kvh, ((T0 >> 4) + kb) & pmask);
-    const size_t bv = vp < 0 ? 0 : block_at(a.p, vp, kvh, ((T0 >> 4) + g) & pmask);
-    const int8_t* s = data + bk * (2 * kKvBlock * HD) + (n & 3) * HD + 16 * g;
+  bool here;
+  auto load_k = [&](int T0, int pg) {
+    const int b0 = (T0 >> 4) + 4 * wave, kb = n >> 2;  // the lane's K rows are block kb's
+    const int kp = __shfl(pg, 4 * wave + kb), vp = __shfl(pg, 4 * wave + g);
+    const size_t bk = block_at(a.p, kp < 0 ? 0 : kp, kvh, (b0 + kb) & pmask);
+    const int8_t* s = data + bk * (2 * kKvBlock * HD) + (n & 3) * HD + (16 * g < HD ? 16 * g : 0);
 #pragma unroll
     for (int tt = 0; tt < 4; tt++)
 #pragma unroll
       for (int c = 0; c < NC; c++)
-        if (HD % 64 == 0 || 64 * c + 16 * g < HD)
-          kr[tt][c] = load16(s + 4 * tt * HD + 64 * c);
-        else
-          kr[tt][c] = make_int4(0, 0, 0, 0);
+        // columns behind the row: the lane's first ones again, against digits of 0
+        kr[tt][c] = load16(s + 4 * tt * HD + (HD % 64 == 0 || 64 * c + 16 * g < HD ? 64 * c : 0));
+    here = vp >= 0;
     sc = make_float2(0.0f, 0.0f);
-    if (vp >= 0) sc = *reinterpret_cast<const float2*>(a.p.scale + 2 * bv);
+    if (here)
+      sc = *reinterpret_cast<const float2*>(a.p.scale + 2 * block_at(a.p, vp, kvh, (b0 + g) & pmask));
   };
-
-  int T0 = tb + wave * kStep;
-  int kp, vp, kp1 = -1, vp1 = -1;
-  if (T0 < te) {
-    pages(T0, &kp, &vp);
-    load_k(T0, kp, vp);
-    pages(T0 + kWaves * kStep, &kp1, &vp1);
-  }
-  for (; T0 < te; T0 += kWaves * kStep) {
-    // V of this step
-    int4 vr[NV];
-    {
-      const size_t bv = vp < 0 ? 0 : block_at(a.p, vp, kvh, ((T0 >> 4) + g) & pmask);
-      const int8_t* s = data + bv * (2 * kKvBlock * HD) + kKvBlock * HD + n * kKvBlock;
+  auto load_v = [&](int T0, int pg) {
 #pragma unroll
-      for (int d = 0; d < NV; d++) vr[d] = load16(s + d * 16 * kKvBlock);
+    for (int s = 0; s < kWaves; s++) {
+      const int vp = __shfl(pg, 4 * s + g);
+      const size_t bv = block_at(a.p, vp < 0 ? 0 : vp, kvh, ((T0 >> 4) + 4 * s + g) & pmask);
+      const int8_t* v = data + bv * (2 * kKvBlock * HD) + kKvBlock * HD + n * kKvBlock;
+      if (T0 + s * kStep < te)
+#pragma unroll
+        for (int d = 0; d < NV; d++)
+          if (HD % 64 == 0 || wave + 4 * d < HD / 16)
+            vr[d][s] = load16(v + (wave + 4 * d) * 16 * kKvBlock);
     }
-    // scores
-    v4i s0[4], s1[4], s2[4];
+  };
+  if (tb < te) {
+    load_k(tb, pg);
+    load_v(tb, pg);
+    pg1 = pages(tb + kRound);
+  }
+
+  // q's digits, for all waves
 #pragma unroll
-    for (int tt = 0; tt < 4; tt++) {
-      s0[tt] = s1[tt] = s2[tt] = v4i{0, 0, 0, 0};
+  for (int i = 0; i < kTurns; i++) {
+    const int at = (i * kWaves + wave) * kSets + lane / kPer;
+    const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    float amax = 0.0f, bad = 0.0f;
 #pragma unroll
-      for (int c = 0; c < NC; c++) {
-        const v4i k = as_v4(kr[tt][c]);
-        s0[tt] = mfma(k, q0[c], s0[tt]);
-        s1[tt] = mfma(k, q1[c], s1[tt]);
-        s2[tt] = mfma(k, q2[c], s2[tt]);
+    for (int j = 0; j < 4; j++) {
+      const float f = fabsf(v[j]);
+      amax = fmaxf(amax, f);
+      bad = f <= 3.402823466e+38f ? bad : 1.0f;
+    }
+#pragma unroll
+    for (int d = 1; d < kPer; d <<= 1) {
+      amax = fmaxf(amax, __shfl_xor(amax, d));
+      bad = fmaxf(bad, __shfl_xor(bad, d));
+    }
+    // below 2^-96 a row's scores are 0 beside any scale of K that fp32 values give
+    amax = fmaxf(amax, 1.2621774e-29f);
+    const float inv = kQMax / amax;
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      u[j] = (uint32_t)((int)rintf(fminf(fmaxf(v[j] * inv, -kQMax), kQMax)) + 0x8080);
+    int e0, e1, e2;
+    digits4(u[0], u[1], u[2], u[3], &e0, &e1, &e2);
+    if (qc < NC * 64) {
+      *reinterpret_cast<int*>(&sq[0][at][qc]) = e0;
+      *reinterpret_cast<int*>(&sq[1][at][qc]) = e1;
+      *reinterpret_cast<int*>(&sq[2][at][qc]) = e2;
+    }
+    if (qc == 0) sqs[at] = bad > 0.0f ? NAN : amax / kQMax * a.scale2;
+  }
+  __syncthreads();
+  float qs[RT];
+#pragma unroll
+  for (int r = 0; r < RT; r++) qs[r] = sqs[16 * r + n];
+
+  float o[RT][NV][4], M[RT], L[RT];
+#pragma unroll
+  for (int r = 0; r < RT; r++) {
+    M[r] = kNone;
+    L[r] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < NV; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[r][d][i] = 0.0f;
+  }
+
+  for (int T0 = tb; T0 < te; T0 += kRound) {
+    const int Tw = T0 + wave * kStep;  // of the wave
+    const bool mine = Tw < te;
+    float e[RT][16], mx[RT];
+    float back = 0.0f, fw = 0.0f;
+#pragma unroll
+    for (int r = 0; r < RT; r++) mx[r] = kNone;
+    if (mine) {
+      // Exponents: scores in powers of two, with V's.
+      const float vs = sc.y;
+      int ev = kMinExp;
+      if (vs > 0x1p-60f) ev = (int)((__builtin_bit_cast(uint32_t, vs) >> 23) & 255) - 127;
+      back = __builtin_bit_cast(float, (uint32_t)(127 - ev) << 23);
+      fw = vs * back * kWMul;
+      const float evf = (float)ev;
+      // Every token of the step seen by every row of the tile?
+      const bool full = __all(here) && Tw + kStep <= t.pos0 + 1 &&
+                        (a.window == 0 || Tw >= t.pos0 + t.queries - a.window);
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+        const float c = qs[r] * sc.x;
+        v4i qd[NC][3];
+#pragma unroll
+        for (int k = 0; k < NC; k++)
+#pragma unroll
+          for (int i = 0; i < 3; i++)
+            qd[k][i] = as_v4(load16(&sq[i][16 * r + n][64 * k + 16 * g]));
+#pragma unroll
+        for (int tt = 0; tt < 4; tt++) {
+          v4i s0 = {0, 0, 0, 0}, s1 = s0, s2 = s0;
+#pragma unroll
+          for (int k = 0; k < NC; k++) {
+            const v4i kk = as_v4(kr[tt][k]);
+            s0 = mfma(kk, qd[k][0], s0);
+            s1 = mfma(kk, qd[k][1], s1);
+            s2 = mfma(kk, qd[k][2], s2);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            e[r][4 * tt + i] = __builtin_fmaf(joined(s2[i], s1[i], s0[i]), c, evf);
+        }
+        if (!full) {
+          const int first = row_lo[r] - (Tw + 16 * g);
+          const unsigned seen = here ? row_hi[r] - row_lo[r] : 0;
+#pragma unroll
+          for (int j = 0; j < 16; j++) e[r][j] = (unsigned)(j - first) < seen ? e[r][j] : kNone;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++) mx[r] = fmaxf(mx[r], e[r][j]);
+        mx[r] = rows_max(mx[r]);
       }
     }
-    const float ks = sc.x, vs = sc.y;
-    const bool here = vp >= 0;
-    const int vblk = T0 + 16 * g;
-    // the next step's K behind this one's V, its pages known a step ahead
-    const int Tn = T0 + kWaves * kStep;
-    vp = vp1;
+    if (g == 0)
+#pragma unroll
+      for (int r = 0; r < RT; r++) smax[wave][r][n] = mx[r];
+    // the next round's K behind this one's V
+    const int Tn = T0 + kRound;
+    const int pgv = pg1;
     if (Tn < te) {
-      load_k(Tn, kp1, vp1);
-      pages(Tn + kWaves * kStep, &kp1, &vp1);
+      load_k(Tn, pg1);
+      pg1 = pages(Tn + kRound);
     }
-    // exponents: scores in powers of two, with V's
-    int ev = kMinExp;
-    if (vs > 0x1p-60f) ev = (int)((__builtin_bit_cast(uint32_t, vs) >> 23) & 255) - 127;
-    const float f = here ? vs * __builtin_bit_cast(float, (uint32_t)(127 - ev) << 23) : 0.0f;
-    const float back = __builtin_bit_cast(float, (uint32_t)(127 - ev) << 23);
-    const float c = qs * ks, evf = (float)ev;
-    float e[16], mx = kNone;
+    __syncthreads();
+    float alpha[RT];
 #pragma unroll
-    for (int tt = 0; tt < 4; tt++)
+    for (int r = 0; r < RT; r++) {
+      const float to = fmaxf(M[r], fmaxf(fmaxf(smax[0][r][n], smax[1][r][n]),
+                                         fmaxf(smax[2][r][n], smax[3][r][n])));
+      const float ref = to == kNone ? 0.0f : to;
+      alpha[r] = lift(M[r], ref);
+      M[r] = to;
+      if (mine) {
+        float sum = 0.0f;
+        int4 p[3];
+        int* d0 = &p[0].x;
+        int* d1 = &p[1].x;
+        int* d2 = &p[2].x;
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int tok = vblk + 4 * tt + i;
-        float v = __builtin_fmaf(joined(s2[tt][i], s1[tt][i], s0[tt][i]), c, evf);
-        if (!(here && tok < row_hi && tok >= row_lo && tok < te)) v = kNone;
-        e[4 * tt + i] = v;
-        mx = fmaxf(mx, v);
+        for (int tt = 0; tt < 4; tt++) {
+          uint32_t u[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float w = __builtin_amdgcn_exp2f(e[r][4 * tt + i] - ref);
+            sum += w;
+            u[i] = __builtin_bit_cast(uint32_t, __builtin_fmaf(w, fw, kWAdd));
+          }
+          digits4(u[0], u[1], u[2], u[3], d0 + tt, d1 + tt, d2 + tt);
+        }
+        L[r] = __builtin_fmaf(sum, back, L[r] * alpha[r]);
+#pragma unroll
+        for (int k = 0; k < 3; k++) sp[wave][r][k][lane] = p[k];
+      } else {
+        L[r] *= alpha[r];
       }
-    mx = rows_max(mx);
-    const float to = fmaxf(M, mx);
-    const float ref = to == kNone ? 0.0f : to;
-    const float alpha = lift(M, ref);
-    M = to;
-    float sum = 0.0f;
-    v4i p0, p1, p2;
-    const float fw = f * kWMul;
-#pragma unroll
-    for (int tt = 0; tt < 4; tt++) {
-      uint32_t u[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float p = __builtin_amdgcn_exp2f(e[4 * tt + i] - ref);
-        sum += p;
-        u[i] = __builtin_bit_cast(uint32_t, __builtin_fmaf(p, fw, kWAdd));
-      }
-      int e0, e1, e2;
-      digits4(u[0], u[1], u[2], u[3], &e0, &e1, &e2);
-      p0[tt] = e0;
-      p1[tt] = e1;
-      p2[tt] = e2;
     }
-    L = __builtin_fmaf(sum, back, L * alpha);
-    // values
+    __syncthreads();
+    // Values: 256 tokens in integers (below 2^22, 2^30 with the next digit).
+    const int steps = (te - T0 + kStep - 1) / kStep;
 #pragma unroll
-    for (int d = 0; d < NV; d++) {
-      const v4i zero = v4i{0, 0, 0, 0}, v = as_v4(vr[d]);
-      const v4i a0 = mfma(v, p0, zero), a1 = mfma(v, p1, zero), a2 = mfma(v, p2, zero);
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        o[d][i] = __builtin_fmaf(o[d][i], alpha, joined(a2[i], a1[i], a0[i]));
-    }
-  }
-  L = rows_sum(L);
-
-  // join the waves: 2 and 3 into 0 and 1, then 1 into 0
-#pragma unroll
-  for (int half = 2; half; half >>= 1) {
-    if (wave >= half && wave < 2 * half) {
+    for (int r = 0; r < RT; r++) {
+      v4i acc[NV][3];
 #pragma unroll
       for (int d = 0; d < NV; d++)
-        *reinterpret_cast<float4*>(&so[wave - half][n][16 * d + 4 * g]) =
-            make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
-      if (g == 0) {
-        sm[wave - half][n][0] = M;
-        sm[wave - half][n][1] = L;
-      }
-    }
-    __syncthreads();
-    if (wave < half) {
-      const float M2 = sm[wave][n][0], L2 = sm[wave][n][1];
-      const float to = fmaxf(M, M2), ref = to == kNone ? 0.0f : to;
-      const float x = lift(M, ref), y = lift(M2, ref);
-      L = L * x + L2 * y;
 #pragma unroll
-      for (int d = 0; d < NV; d++) {
-        const float4 w = *reinterpret_cast<const float4*>(&so[wave][n][16 * d + 4 * g]);
-        o[d][0] = o[d][0] * x + w.x * y;
-        o[d][1] = o[d][1] * x + w.y * y;
-        o[d][2] = o[d][2] * x + w.z * y;
-        o[d][3] = o[d][3] * x + w.w * y;
-      }
-      M = to;
+        for (int k = 0; k < 3; k++) acc[d][k] = v4i{0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < kWaves; s++)
+        if (s < steps) {
+          v4i w[3];
+#pragma unroll
+          for (int k = 0; k < 3; k++) w[k] = as_v4(sp[s][r][k][lane]);
+#pragma unroll
+          for (int d = 0; d < NV; d++)
+            if (HD % 64 == 0 || wave + 4 * d < HD / 16)
+#pragma unroll
+              for (int k = 0; k < 3; k++) acc[d][k] = mfma(as_v4(vr[d][s]), w[k], acc[d][k]);
+        }
+#pragma unroll
+      for (int d = 0; d < NV; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          o[r][d][i] =
+              __builtin_fmaf(o[r][d][i], alpha[r], joined(acc[d][2][i], acc[d][1][i], acc[d][0][i]));
     }
-    __syncthreads();
+    if (Tn < te) load_v(Tn, pgv);
   }
-  if (wave != 0 || !row_ok) return;
-  if (a.splits == 1) {
-    // a row that saw nothing: L = 0
-    const float inv = L == 0.0f ? 0.0f : 1.0f / (L * kWMul);
-    float* dst = a.out + row * a.out_stride + (long)head * HD + 4 * g;
+
+  // The waves' denominators; then each wave has its columns' results.
 #pragma unroll
-    for (int d = 0; d < NV; d++)
-      *reinterpret_cast<float4*>(dst + 16 * d) =
-          make_float4(o[d][0] * inv, o[d][1] * inv, o[d][2] * inv, o[d][3] * inv);
-  } else {
-    const size_t at = ((size_t)(slot * gridDim.y + hy) * a.splits + z) * kRows + n;
+  for (int r = 0; r < RT; r++) {
+    L[r] = rows_sum(L[r]);
+    if (g == 0) ssum[wave][r][n] = L[r];
+  }
+  __syncthreads();
 #pragma unroll
-    for (int d = 0; d < NV; d++)
-      *reinterpret_cast<float4*>(a.part + at * HD + 16 * d + 4 * g) =
-          make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
-    if (g == 0) {
-      a.ml[2 * at] = M;
-      a.ml[2 * at + 1] = L;
+  for (int r = 0; r < RT; r++) {
+    if (!row_ok[r]) continue;
+    const float l = (ssum[0][r][n] + ssum[1][r][n]) + (ssum[2][r][n] + ssum[3][r][n]);
+    if (a.splits == 1) {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / (l * kWMul);  // 0: a row that saw nothing
+      float* dst = a.out + row[r] * a.out_stride + (long)head[r] * HD + 4 * g;
+#pragma unroll
+      for (int d = 0; d < NV; d++)
+        if (HD % 64 == 0 || wave + 4 * d < HD / 16)
+          *reinterpret_cast<float4*>(dst + 16 * (wave + 4 * d)) = make_float4(
+              o[r][d][0] * inv, o[r][d][1] * inv, o[r][d][2] * inv, o[r][d][3] * inv);
+    } else {
+      const size_t at =
+          ((size_t)(slot * gridDim.y + hy) * a.splits + z) * (16 * RT) + 16 * r + n;
+#pragma unroll
+      for (int d = 0; d < NV; d++)
+        if (HD % 64 == 0 || wave + 4 * d < HD / 16)
+          *reinterpret_cast<float4*>(a.part + at * HD + 16 * (wave + 4 * d) + 4 * g) =
+              make_float4(o[r][d][0], o[r][d][1], o[r][d][2], o[r][d][3]);
+      if (wave == 0 && g == 0)
+        *reinterpret_cast<float2*>(a.ml + 2 * at) = make_float2(M[r], l);
     }
   }
 }
 
-// The parts of each row joined: a workgroup per row, a thread per column (and
-// a group of threads per part where columns leave some).
+// The parts of each row joined: a workgroup per row.  Its threads first form
+// the parts' weights 2^(m_s - M), a part each, then take four columns of a part each,
+// as many parts side by side as there are threads for, four loads in flight.
 template <int HD>
 __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
-  __shared__ float red[256];
-  const int n = blockIdx.x % kRows, slot = blockIdx.x / kRows, hy = blockIdx.y;
+  constexpr int Q = HD / 4, G = 256 / Q;
+  __shared__ float weight[kMaxParts];
+  __shared__ float red[8];
+  __shared__ float sums[G][HD];
+  const int rows = 16 * a.rt;
+  const int n = blockIdx.x % rows, slot = blockIdx.x / rows, hy = blockIdx.y;
   const Tile t = tile_of(a, slot);
   const int qi = n / a.hpt, hh = hy % a.hgroups * a.hpt + n % a.hpt;
   if (!(qi < t.queries && hh < a.group)) return;
@@ -423,62 +498,108 @@ __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
     parts = (int)(((long)hi - lo + a.chunk - 1) / a.chunk);
     if (parts > a.splits) parts = a.splits;
   }
-  const size_t at = (size_t)(slot * gridDim.y + hy) * a.splits * kRows + n;
-  float M = kNone;
-  for (int s = threadIdx.x; s < parts; s += 256) M = fmaxf(M, a.ml[2 * (at + (size_t)s * kRows)]);
+  const size_t at = (size_t)(slot * gridDim.y + hy) * a.splits * rows + n;
+  const int tid = threadIdx.x;
+  constexpr int kEach = kMaxParts / 256;
+  float m[kEach], l[kEach], M = kNone, L = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kEach; j++) {
+    const int s = tid + 256 * j;
+    m[j] = kNone;
+    l[j] = 0.0f;
+    if (s < parts) {
+      const float2 v = *reinterpret_cast<const float2*>(a.ml + 2 * (at + (size_t)s * rows));
+      m[j] = v.x;
+      l[j] = v.y;
+    }
+    M = fmaxf(M, m[j]);
+  }
+  // the first parts' values on their way meanwhile
+  const int c = tid % Q, grp = tid / Q;
+  const float* part = a.part + at * HD + 4 * c;
+  constexpr int kAhead = 4;
+  float4 v[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; j++) {
+    const int s = grp + j * G;
+    v[j] = make_float4(0, 0, 0, 0);
+    if (grp < G && s < parts) v[j] = *reinterpret_cast<const float4*>(part + (size_t)s * rows * HD);
+  }
   for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = M;
+  if ((tid & 63) == 0) red[tid >> 6] = M;
   __syncthreads();
   M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float ref = M == kNone ? 0.0f : M;
-  __syncthreads();
-  constexpr int kGroups = 256 / HD > 0 ? 256 / HD : 1;
-  const int c = threadIdx.x % HD, grp = threadIdx.x / HD;
-  float sum = 0.0f, L = 0.0f;
-  if (grp < kGroups)
-    for (int s = grp; s < parts; s += kGroups) {
-      const size_t r = at + (size_t)s * kRows;
-      const float w = lift(a.ml[2 * r], ref);
-      sum += w * a.part[r * HD + c];
-      L += w * a.ml[2 * r + 1];
-    }
-  if (kGroups > 1) {
-    __shared__ float redl[256];
-    red[threadIdx.x] = sum;
-    redl[threadIdx.x] = L;
-    __syncthreads();
-    if (grp == 0)
-      for (int j = 1; j < kGroups; j++) {
-        sum += red[j * HD + c];
-        L += redl[j * HD + c];
-      }
+#pragma unroll
+  for (int j = 0; j < kEach; j++) {
+    const float w = lift(m[j], ref);
+    weight[tid + 256 * j] = w;
+    L += w * l[j];
   }
-  if (grp == 0)
-    a.out[(t.row0 + qi) * a.out_stride + (long)(hy / a.hgroups * a.group + hh) * HD + c] =
+  for (int d = 32; d; d >>= 1) L += __shfl_xor(L, d);
+  if ((tid & 63) == 0) red[4 + (tid >> 6)] = L;
+  __syncthreads();
+  L = (red[4] + red[5]) + (red[6] + red[7]);
+  float4 o = make_float4(0, 0, 0, 0);
+  if (grp < G) {
+    for (int s0 = grp; s0 < parts; s0 += kAhead * G) {
+      float4 u[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; j++) {
+        const int s = s0 + (kAhead + j) * G;
+        u[j] = make_float4(0, 0, 0, 0);
+        if (s < parts) u[j] = *reinterpret_cast<const float4*>(part + (size_t)s * rows * HD);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; j++) {
+        const int s = s0 + j * G;
+        const float w = s < parts ? weight[s] : 0.0f;
+        o.x += w * v[j].x;
+        o.y += w * v[j].y;
+        o.z += w * v[j].z;
+        o.w += w * v[j].w;
+        v[j] = u[j];
+      }
+    }
+    *reinterpret_cast<float4*>(&sums[grp][4 * c]) = o;
+  }
+  __syncthreads();
+  if (tid < HD) {
+    float sum = 0.0f;
+    for (int j = 0; j < G; j++) sum += sums[j][tid];
+    a.out[(t.row0 + qi) * a.out_stride + (long)(hy / a.hgroups * a.group + hh) * HD + tid] =
         L == 0.0f ? 0.0f : sum / (L * kWMul);
+  }
 }
 
 // How the work is cut.  Heads: at most 16 of a kv head's query heads share a
-// tile, as many queries beside each other as fill it.  Tokens: a tile's part is
-// one workgroup; there are as many parts as it takes to have four workgroups
-// per CU (two are resident; lengths differ), each of 256 tokens or more.
+// tile, as many queries beside each other as fill it; 32 rows where sequences bring
+// as many.  Tokens: a tile's part is one workgroup; there are as many parts as
+// it takes to have four workgroups per CU (lengths differ), each of a round or more.
 AttnArgs attn_plan(const PoolView& p, const Ragged& r, int n_heads, int max_len, int window) {
   AttnArgs a = {};
   a.p = p;
   a.r = r;
   a.n_heads = n_heads;
   a.group = n_heads / p.n_kv_heads;
-  a.hgroups = (a.group + kRows - 1) / kRows;
+  a.hgroups = (a.group + 15) / 16;
   a.hpt = (a.group + a.hgroups - 1) / a.hgroups;
-  a.qpt = kRows / a.hpt;
+  a.rt = p.hd <= 128 && (long)r.T * a.hpt >= 32l * r.n ? 2 : 1;
+  a.qpt = 16 * a.rt / a.hpt;
+  a.extra = 1;
+  if (r.T <= r.n) {  // one row a sequence: a tile for each row, and no slot to spare
+    a.qpt = 1;
+    a.extra = 0;
+  }
   a.window = window;
-  a.slots = r.T / a.qpt + r.n;
+  a.slots = r.T / a.qpt + a.extra * r.n;
   long range = max_len;
   if (window > 0 && window + (long)a.qpt + kStep < range) range = window + (long)a.qpt + kStep;
   const long tiles = (r.T / a.qpt > r.n ? r.T / a.qpt : r.n) * (long)p.n_kv_heads * a.hgroups;
-  long splits = (1024 + tiles - 1) / tiles;
-  const long most = (range + 4 * kStep - 1) / (4 * kStep);
+  long splits = tiles >= 384 ? 1 : (1024 + tiles - 1) / tiles;
+  const long most = (range + kRound - 1) / kRound;
   if (splits > most) splits = most;
+  if (splits > kMaxParts) splits = kMaxParts;
   if (splits < 1) splits = 1;
   long chunk = (range + splits - 1) / splits;
   chunk = (chunk + kStep - 1) / kStep * kStep;
@@ -487,8 +608,19 @@ AttnArgs attn_plan(const PoolView& p, const Ragged& r, int n_heads, int max_len,
   return a;
 }
 
-size_t part_floats(const AttnArgs& a) {
-  return (size_t)a.slots * a.p.n_kv_heads * a.hgroups * a.splits * kRows;
+// Rows of all parts.
+size_t part_rows(const AttnArgs& a) {
+  return (size_t)a.slots * a.p.n_kv_heads * a.hgroups * a.splits * (16 * a.rt);
+}
+
+template <int HD>
+void attn_launch(const AttnArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)(a.slots * a.splits), (unsigned)(a.p.n_kv_heads * a.hgroups));
+  if (a.rt == 1) hipLaunchKernelGGL((k_pool_attn<HD, 1>), grid, dim3(256), 0, st, a);
+  if constexpr (HD <= 128)
+    if (a.rt == 2) hipLaunchKernelGGL((k_pool_attn<HD, 2>), grid, dim3(256), 0, st, a);
+  if (a.splits > 1)
+    hipLaunchKernelGGL(k_pool_attn_join<HD>, dim3(16 * a.rt * a.slots, grid.y), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -496,7 +628,7 @@ size_t part_floats(const AttnArgs& a) {
 size_t kv_attention_scratch(const PoolView& p, const Ragged& r, int n_heads, int max_len,
                             int window) {
   const AttnArgs a = attn_plan(p, r, n_heads, max_len, window);
-  return a.splits == 1 ? 0 : part_floats(a) * (p.hd + 2) * sizeof(float);
+  return a.splits == 1 ? 0 : part_rows(a) * (p.hd + 2) * sizeof(float);
 }
 
 hipError_t kv_attention_launch(const PoolView& p, const Ragged& r, int n_heads, const float* q,
@@ -509,25 +641,17 @@ hipError_t kv_attention_launch(const PoolView& p, const Ragged& r, int n_heads, 
   a.out_stride = out_stride;
   a.scale2 = scale * 1.44269504088896340736f;
   a.part = static_cast<float*>(work);
-  a.ml = a.part + part_floats(a) * p.hd;
-  const dim3 grid((unsigned)(a.slots * a.splits), (unsigned)(p.n_kv_heads * a.hgroups));
-#define ATTN(HD)                                                                               \
-  {                                                                                            \
-    hipLaunchKernelGGL(k_pool_attn<HD>, grid, dim3(256), 0, st, a);                            \
-    if (a.splits > 1)                                                                          \
-      hipLaunchKernelGGL(k_pool_attn_join<HD>, dim3(kRows * a.slots, grid.y), dim3(256), 0, st, a); \
-  }
+  a.ml = a.part + part_rows(a) * p.hd;
   switch (p.hd) {
-    case 32: ATTN(32) break;
-    case 64: ATTN(64) break;
-    case 96: ATTN(96) break;
-    case 128: ATTN(128) break;
-    case 160: ATTN(160) break;
-    case 192: ATTN(192) break;
-    case 224: ATTN(224) break;
-    default: ATTN(256) break;
+    case 32: attn_launch<32>(a, st); break;
+    case 64: attn_launch<64>(a, st); break;
+    case 96: attn_launch<96>(a, st); break;
+    case 128: attn_launch<128>(a, st); break;
+    case 160: attn_launch<160>(a, st); break;
+    case 192: attn_launch<192>(a, st); break;
+    case 224: attn_launch<224>(a, st); break;
+    default: attn_launch<256>(a, st); break;
   }
-#undef ATTN
   return hipGetLastError();
 }
 

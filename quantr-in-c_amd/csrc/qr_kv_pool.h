@@ -40,45 +40,61 @@ __device__ inline int ragged_start(const Ragged& r, int i) {
   return s < 0 ? 0 : s > r.T ? r.T : s;
 }
 
-// Sequence i's row of the table, its rows and its length (0 where the row of
-// the table does not exist).
+// A sequence of the batch: its row of the table, its rows and its length (0
+// where that row of the table does not exist).
 struct SeqRows {
   int seq, row0, m, len;
 };
-__device__ inline SeqRows seq_rows(const PoolView& p, const Ragged& r, int i) {
-  SeqRows s;
-  s.row0 = ragged_start(r, i);
-  s.m = ragged_start(r, i + 1) - s.row0;
-  if (s.m < 0) s.m = 0;
-  s.seq = r.seqs ? r.seqs[i] : i;
-  if ((unsigned)s.seq >= (unsigned)p.n_seqs) {
-    s.seq = 0;
-    s.len = 0;
-    return s;
-  }
-  const long cap = (long)p.max_pages << p.page_shift;
-  const int n = p.len[s.seq];
-  s.len = n < 0 ? 0 : n > cap ? (int)cap : n;
-  return s;
-}
 
 // Which sequence a slot serves, where each sequence's rows are cut into pieces
 // of q rows: sequence i has the slots from start[i] / q + extra * i on.  There
 // are never fewer than its pieces (floor(b / q) - floor(a / q) + 1 >=
 // ceil((b - a) / q)), so the host sizes the grid by T / q + extra * n without
-// knowing the lengths, and a slot without a piece ends.  Returns the sequence
-// and sets *piece.
-__device__ inline int slot_seq(const Ragged& r, int slot, int q, int extra, int* piece) {
-  int lo = 0, hi = r.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (ragged_start(r, mid) / q + extra * mid <= slot)
-      lo = mid;
-    else
-      hi = mid - 1;
+// knowing the lengths, and a slot without a piece ends.  *piece: which of the
+// sequence's slots this is, < 0 for none.
+//
+// All lanes of the wave search at once, 64 places a step, and what is needed of
+// the place is loaded beside it: up to 64 sequences take two dependent
+// loads (a binary search took one for each of its steps, 5 us of a launch over 32).
+__device__ inline SeqRows slot_rows(const PoolView& p, const Ragged& r, int slot, int q, int extra,
+                                    int* piece) {
+  const int lane = (int)(threadIdx.x & 63);
+  int lo = 0, count = r.n, at, first, next, seq;
+  unsigned long long below;
+  for (;;) {
+    const int step = (count + 63) >> 6;
+    at = lo + lane * step;
+    const bool in = lane * step < count;
+    if (!in) at = lo;
+    first = ragged_start(r, at);
+    next = 0;
+    seq = at;
+    if (step == 1) {
+      next = ragged_start(r, at + 1);
+      if (r.seqs) seq = r.seqs[at];
+    }
+    below = __ballot(in && first / q + extra * at <= slot);
+    const int k = below ? 63 - __builtin_clzll(below) : 0;
+    if (step == 1) {
+      SeqRows s;
+      s.row0 = __builtin_amdgcn_readlane(first, k);
+      s.m = __builtin_amdgcn_readlane(next, k) - s.row0;
+      if (s.m < 0) s.m = 0;
+      s.seq = __builtin_amdgcn_readlane(seq, k);
+      *piece = slot - (s.row0 / q + extra * (lo + k));
+      s.len = 0;
+      if ((unsigned)s.seq >= (unsigned)p.n_seqs) {
+        s.seq = 0;
+        return s;
+      }
+      const long cap = (long)p.max_pages << p.page_shift;
+      const int n = p.len[s.seq];
+      s.len = n < 0 ? 0 : n > cap ? (int)cap : n;
+      return s;
+    }
+    lo += k * step;
+    count = count - k * step < step ? count - k * step : step;
   }
-  *piece = slot - (ragged_start(r, lo) / q + extra * lo);
-  return lo;
 }
 
 // The physical page of a sequence's logical page, -1 where there is none.

@@ -409,8 +409,7 @@ struct BlockRows {
 __device__ inline BlockRows block_rows(const PoolView& p, const Ragged& r, int slot, int kvh) {
   BlockRows b;
   b.any = b.there = false;
-  const int i = slot_seq(r, slot, kKvBlock, 2, &b.piece);
-  b.s = seq_rows(p, r, i);
+  b.s = slot_rows(p, r, slot, kKvBlock, 2, &b.piece);
   if (b.piece < 0 || b.s.m == 0) return b;
   const int pos0 = b.s.len - b.s.m;  // of the first row; < 0 where there are more rows than tokens
   const long lb = (long)(pos0 < 0 ? 0 : pos0) / kKvBlock + b.piece;
