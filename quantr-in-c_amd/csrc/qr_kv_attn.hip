@@ -25,7 +25,7 @@
 // The values' columns are what the waves share out: each reads all four waves'
 // digits from LDS (12 KiB) and sums 256 tokens in integers before anything is
 // rounded.  A wave that kept all columns of its own tokens instead converted four
-// times as many sums, held 206 registers for 142, and ended in a join of the waves.
+// times as many sums, held 206 registers for 168, and ended in a join of the waves.
 //
 // The weights carry V's scale: with vs = f 2^e (1 <= f < 2), w_t = f 2^(s_t
 // log2(e) + e - M) against the running maximum M of the exponents, so the
@@ -43,7 +43,9 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 constexpr int kStep = 64;   // tokens of a wave's step
 constexpr int kWaves = 4;   // of a workgroup
 constexpr int kRound = kStep * kWaves;
+constexpr int kPages = 1024;  // blocks whose pages are held at a time: 64 rounds
 constexpr int kMaxParts = 1024;  // of a tile's tokens
+constexpr int kJoinWave = 16;    // up to as many one wave joins a row
 constexpr float kNone = -INFINITY;
 // Weights below 2 become whole numbers below 2^23 - 0x8080: added to 2^23 +
 // 0x8080 they are the low mantissa bits of a float, and its three low bytes the
@@ -78,17 +80,17 @@ struct AttnArgs {
   float scale2;         // scale * log2(e)
   float* part;          // [tile, head][splits][row][hd], then [..][row][2]
   float* ml;
+  int4* meta;           // [tile]: first row, queries, parts
 };
 
 __device__ inline Tile tile_of(const AttnArgs& a, int slot) {
   Tile t;
-  t.queries = 0;
   int piece;
   const SeqRows s = slot_rows(a.p, a.r, slot, a.qpt, a.extra, &piece);
   const int at = piece * a.qpt;
-  if (piece < 0 || at >= s.m) return t;
   t.row0 = s.row0 + at;
   t.queries = s.m - at < a.qpt ? s.m - at : a.qpt;
+  if (piece < 0 || at >= s.m) t.queries = 0;
   t.seq = s.seq;
   t.len = s.len;
   t.pos0 = s.len - s.m + at;
@@ -173,6 +175,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
   __shared__ int4 sp[kWaves][RT][3][64];        // the weights' digits
   __shared__ int8_t sq[3][16 * RT][NC * 64 + 16];  // the rows' digits
   __shared__ float sqs[16 * RT];                   // and what one of the last place stands for
+  __shared__ int spg[kPages];
   __shared__ float smax[kWaves][RT][16];
   __shared__ float ssum[kWaves][RT][16];
   const int lane = threadIdx.x & 63;
@@ -183,20 +186,29 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
   const int hy = blockIdx.y;
   const int kvh = hy / a.hgroups, hg = hy % a.hgroups;
   const Tile t = tile_of(a, slot);
-  if (t.queries == 0) return;
+  // Pages of a round's 16 blocks, one in each lane group's lanes; -1: none.
+  auto pages = [&](int T0) { return page_at(a.p, t.seq, (T0 + 16 * n) >> a.p.page_shift); };
+  // The first round's, where no window moves it, before the length is there.
+  int pg = -1;
+  if (a.window == 0) pg = pages(z * a.chunk);
   int lo, hi, tb, te;
   tile_range(a, t, &lo, &hi);
   part_range(a, lo, hi, z, &tb, &te);
-  if (tb >= te && a.splits > 1) return;  // the joining launch skips it too
-
-  // Pages of a round's 16 blocks, one in each lane group's lanes; -1: none.
-  auto pages = [&](int T0) {
-    const int tok = T0 + 16 * n;
-    return tok < te ? page_at(a.p, t.seq, tok >> a.p.page_shift) : -1;
+  if (a.splits > 1 && z == 0 && hy == 0 && threadIdx.x == 0)  // for the joining launch
+    a.meta[slot] = make_int4(t.row0, t.queries, hi > lo ? (hi - lo - 1) / a.chunk + 1 : 0, 0);
+  if (t.queries == 0 || (tb >= te && a.splits > 1)) return;
+  if (a.window > 0) pg = pages(tb);
+  if (tb + 16 * n >= te) pg = -1;
+  // Those of later rounds by way of LDS, kPages blocks at a time: a load of them in the
+  // loop would wait for the V before it.
+  auto fill_pages = [&](int T0) {
+    for (int i = threadIdx.x; i < kPages && T0 + 16 * i < te; i += 256)
+      spg[i] = page_at(a.p, t.seq, (T0 + 16 * i) >> a.p.page_shift);
   };
+  const bool more = tb + kRound < te;
+  if (more) fill_pages(tb);
   const int pmask = (1 << (a.p.page_shift - 4)) - 1;
   const int8_t* const data = a.p.data;
-  int pg = pages(tb), pg1 = -1;
 
   // this lane's rows
   long row[RT];
@@ -233,9 +245,10 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
   int4 kr[4][NC], vr[NV][kWaves];
   float2 sc;
   bool here;
-  auto load_k = [&](int T0, int pg) {
-    const int b0 = (T0 >> 4) + 4 * wave, kb = n >> 2;  // the lane's K rows are block kb's
-    const int kp = __shfl(pg, 4 * wave + kb), vp = __shfl(pg, 4 * wave + g);
+  const int kb = 4 * wave + (n >> 2);  // the round's block of the lane's K rows
+  int kp = -1, wp = -1, vp[kWaves];  // pages of its K, its scales, and V's four blocks
+  auto load_k = [&](int T0) {
+    const int b0 = T0 >> 4;
     const size_t bk = block_at(a.p, kp < 0 ? 0 : kp, kvh, (b0 + kb) & pmask);
     const int8_t* s = data + bk * (2 * kKvBlock * HD) + (n & 3) * HD + (16 * g < HD ? 16 * g : 0);
 #pragma unroll
@@ -244,28 +257,29 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
       for (int c = 0; c < NC; c++)
         // columns behind the row: the lane's first ones again, against digits of 0
         kr[tt][c] = load16(s + 4 * tt * HD + (HD % 64 == 0 || 64 * c + 16 * g < HD ? 64 * c : 0));
-    here = vp >= 0;
+    here = wp >= 0;
     sc = make_float2(0.0f, 0.0f);
     if (here)
-      sc = *reinterpret_cast<const float2*>(a.p.scale + 2 * block_at(a.p, vp, kvh, (b0 + g) & pmask));
+      sc = *reinterpret_cast<const float2*>(
+          a.p.scale + 2 * block_at(a.p, wp, kvh, (b0 + 4 * wave + g) & pmask));
   };
-  auto load_v = [&](int T0, int pg) {
+  auto load_v = [&](int T0) {
 #pragma unroll
     for (int s = 0; s < kWaves; s++) {
-      const int vp = __shfl(pg, 4 * s + g);
-      const size_t bv = block_at(a.p, vp < 0 ? 0 : vp, kvh, ((T0 >> 4) + 4 * s + g) & pmask);
+      const size_t bv = block_at(a.p, vp[s] < 0 ? 0 : vp[s], kvh, ((T0 >> 4) + 4 * s + g) & pmask);
       const int8_t* v = data + bv * (2 * kKvBlock * HD) + kKvBlock * HD + n * kKvBlock;
-      if (T0 + s * kStep < te)
 #pragma unroll
-        for (int d = 0; d < NV; d++)
-          if (HD % 64 == 0 || wave + 4 * d < HD / 16)
-            vr[d][s] = load16(v + (wave + 4 * d) * 16 * kKvBlock);
+      for (int d = 0; d < NV; d++)
+        if (HD % 64 == 0 || wave + 4 * d < HD / 16)
+          vr[d][s] = load16(v + (wave + 4 * d) * 16 * kKvBlock);
     }
   };
   if (tb < te) {
-    load_k(tb, pg);
-    load_v(tb, pg);
-    pg1 = pages(tb + kRound);
+    kp = __shfl(pg, kb);
+    wp = __shfl(pg, 4 * wave + g);
+#pragma unroll
+    for (int s = 0; s < kWaves; s++) vp[s] = __shfl(pg, 4 * s + g);
+    load_k(tb);
   }
 
   // q's digits, for all waves
@@ -372,12 +386,22 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     if (g == 0)
 #pragma unroll
       for (int r = 0; r < RT; r++) smax[wave][r][n] = mx[r];
-    // the next round's K behind this one's V
+    // This round's V, and behind it the next one's K.
+    load_v(T0);
     const int Tn = T0 + kRound;
-    const int pgv = pg1;
     if (Tn < te) {
-      load_k(Tn, pg1);
-      pg1 = pages(Tn + kRound);
+      const int at = (Tn - tb) >> 4 & (kPages - 1);
+      if (at == 0) {
+        __syncthreads();
+        fill_pages(Tn);
+        __syncthreads();
+      }
+      const int left = (te - Tn + 15) >> 4;  // blocks
+      kp = kb < left ? spg[at + kb] : -1;
+      wp = 4 * wave + g < left ? spg[at + 4 * wave + g] : -1;
+#pragma unroll
+      for (int s = 0; s < kWaves; s++) vp[s] = 4 * s + g < left ? spg[at + 4 * s + g] : -1;
+      load_k(Tn);
     }
     __syncthreads();
     float alpha[RT];
@@ -409,12 +433,14 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
 #pragma unroll
         for (int k = 0; k < 3; k++) sp[wave][r][k][lane] = p[k];
       } else {
+        // no tokens: digits of 0, whatever V holds there
         L[r] *= alpha[r];
+#pragma unroll
+        for (int k = 0; k < 3; k++) sp[wave][r][k][lane] = make_int4(0, 0, 0, 0);
       }
     }
     __syncthreads();
     // Values: 256 tokens in integers (below 2^22, 2^30 with the next digit).
-    const int steps = (te - T0 + kStep - 1) / kStep;
 #pragma unroll
     for (int r = 0; r < RT; r++) {
       v4i acc[NV][3];
@@ -423,17 +449,16 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
 #pragma unroll
         for (int k = 0; k < 3; k++) acc[d][k] = v4i{0, 0, 0, 0};
 #pragma unroll
-      for (int s = 0; s < kWaves; s++)
-        if (s < steps) {
-          v4i w[3];
+      for (int s = 0; s < kWaves; s++) {
+        v4i w[3];
 #pragma unroll
-          for (int k = 0; k < 3; k++) w[k] = as_v4(sp[s][r][k][lane]);
+        for (int k = 0; k < 3; k++) w[k] = as_v4(sp[s][r][k][lane]);
 #pragma unroll
-          for (int d = 0; d < NV; d++)
-            if (HD % 64 == 0 || wave + 4 * d < HD / 16)
+        for (int d = 0; d < NV; d++)
+          if (HD % 64 == 0 || wave + 4 * d < HD / 16)
 #pragma unroll
-              for (int k = 0; k < 3; k++) acc[d][k] = mfma(as_v4(vr[d][s]), w[k], acc[d][k]);
-        }
+            for (int k = 0; k < 3; k++) acc[d][k] = mfma(as_v4(vr[d][s]), w[k], acc[d][k]);
+      }
 #pragma unroll
       for (int d = 0; d < NV; d++)
 #pragma unroll
@@ -441,7 +466,6 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
           o[r][d][i] =
               __builtin_fmaf(o[r][d][i], alpha[r], joined(acc[d][2][i], acc[d][1][i], acc[d][0][i]));
     }
-    if (Tn < te) load_v(Tn, pgv);
   }
 
   // The waves' denominators; then each wave has its columns' results.
@@ -477,98 +501,115 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
   }
 }
 
-// The parts of each row joined: a workgroup per row.  Its threads first form
-// the parts' weights 2^(m_s - M), a part each, then take four columns of a part each,
-// as many parts side by side as there are threads for, four loads in flight.
-template <int HD>
+// The parts of each row joined, by W waves a row: one where parts are few (a
+// workgroup then joins four rows), four where one wave would be left with long loops.  The
+// loads are of addresses that the grid alone gives, all at once: the first part's
+// workgroup left the tile's rows and number of parts.
+template <int HD, int W>
 __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
-  constexpr int Q = HD / 4, G = 256 / Q;
-  __shared__ float weight[kMaxParts];
+  constexpr int Q = HD / 4, G = 64 * W / Q;  // threads of a part's columns, parts side by side
+  constexpr int kEach = W == 1 ? 1 : kMaxParts / 256, kAhead = W == 1 ? 8 : 4;
+  __shared__ float weight[W == 1 ? 1 : kMaxParts];
   __shared__ float red[8];
-  __shared__ float sums[G][HD];
-  const int rows = 16 * a.rt;
-  const int n = blockIdx.x % rows, slot = blockIdx.x / rows, hy = blockIdx.y;
-  const Tile t = tile_of(a, slot);
-  const int qi = n / a.hpt, hh = hy % a.hgroups * a.hpt + n % a.hpt;
-  if (!(qi < t.queries && hh < a.group)) return;
-  int lo, hi;
-  tile_range(a, t, &lo, &hi);
-  int parts = 0;
-  if (hi > lo) {
-    parts = (int)(((long)hi - lo + a.chunk - 1) / a.chunk);
-    if (parts > a.splits) parts = a.splits;
-  }
+  __shared__ float sums[W == 1 ? 1 : G][HD];
+  const int rows = 16 * a.rt, tid = threadIdx.x % (64 * W);
+  const int item = blockIdx.x * (4 / W) + threadIdx.x / (64 * W);
+  const int n = item % rows, slot = item / rows, hy = blockIdx.y;
   const size_t at = (size_t)(slot * gridDim.y + hy) * a.splits * rows + n;
-  const int tid = threadIdx.x;
-  constexpr int kEach = kMaxParts / 256;
-  float m[kEach], l[kEach], M = kNone, L = 0.0f;
+  const int4 meta = a.meta[slot];
+  float m[kEach], l[kEach];
 #pragma unroll
   for (int j = 0; j < kEach; j++) {
     const int s = tid + 256 * j;
-    m[j] = kNone;
-    l[j] = 0.0f;
-    if (s < parts) {
-      const float2 v = *reinterpret_cast<const float2*>(a.ml + 2 * (at + (size_t)s * rows));
-      m[j] = v.x;
-      l[j] = v.y;
-    }
-    M = fmaxf(M, m[j]);
+    float2 v = make_float2(kNone, 0.0f);
+    if (s < a.splits) v = *reinterpret_cast<const float2*>(a.ml + 2 * (at + (size_t)s * rows));
+    m[j] = v.x;
+    l[j] = v.y;
   }
-  // the first parts' values on their way meanwhile
   const int c = tid % Q, grp = tid / Q;
   const float* part = a.part + at * HD + 4 * c;
-  constexpr int kAhead = 4;
   float4 v[kAhead];
 #pragma unroll
   for (int j = 0; j < kAhead; j++) {
     const int s = grp + j * G;
     v[j] = make_float4(0, 0, 0, 0);
-    if (grp < G && s < parts) v[j] = *reinterpret_cast<const float4*>(part + (size_t)s * rows * HD);
+    if (grp < G && s < a.splits)
+      v[j] = *reinterpret_cast<const float4*>(part + (size_t)s * rows * HD);
   }
-  for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
-  if ((tid & 63) == 0) red[tid >> 6] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float ref = M == kNone ? 0.0f : M;
+  const int qi = n / a.hpt, hh = hy % a.hgroups * a.hpt + n % a.hpt;
+  if (!(qi < meta.y && hh < a.group)) return;
+  const int parts = meta.z < a.splits ? meta.z : a.splits;
+  float M = kNone, L = 0.0f;
 #pragma unroll
   for (int j = 0; j < kEach; j++) {
-    const float w = lift(m[j], ref);
-    weight[tid + 256 * j] = w;
-    L += w * l[j];
+    if (tid + 256 * j >= parts) m[j] = kNone;  // a part that is not there holds anything
+    M = fmaxf(M, m[j]);
+  }
+  for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
+  if (W > 1) {
+    if ((tid & 63) == 0) red[tid >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  }
+  const float ref = M == kNone ? 0.0f : M;
+  float w[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; j++) {
+    w[j] = lift(m[j], ref);
+    if (W > 1) weight[tid + 256 * j] = w[j];
+    if (m[j] != kNone) L += w[j] * l[j];
   }
   for (int d = 32; d; d >>= 1) L += __shfl_xor(L, d);
-  if ((tid & 63) == 0) red[4 + (tid >> 6)] = L;
-  __syncthreads();
-  L = (red[4] + red[5]) + (red[6] + red[7]);
-  float4 o = make_float4(0, 0, 0, 0);
-  if (grp < G) {
-    for (int s0 = grp; s0 < parts; s0 += kAhead * G) {
-      float4 u[kAhead];
-#pragma unroll
-      for (int j = 0; j < kAhead; j++) {
-        const int s = s0 + (kAhead + j) * G;
-        u[j] = make_float4(0, 0, 0, 0);
-        if (s < parts) u[j] = *reinterpret_cast<const float4*>(part + (size_t)s * rows * HD);
-      }
-#pragma unroll
-      for (int j = 0; j < kAhead; j++) {
-        const int s = s0 + j * G;
-        const float w = s < parts ? weight[s] : 0.0f;
-        o.x += w * v[j].x;
-        o.y += w * v[j].y;
-        o.z += w * v[j].z;
-        o.w += w * v[j].w;
-        v[j] = u[j];
-      }
-    }
-    *reinterpret_cast<float4*>(&sums[grp][4 * c]) = o;
+  if (W > 1) {
+    if ((tid & 63) == 0) red[4 + (tid >> 6)] = L;
+    __syncthreads();
+    L = (red[4] + red[5]) + (red[6] + red[7]);
   }
-  __syncthreads();
-  if (tid < HD) {
-    float sum = 0.0f;
-    for (int j = 0; j < G; j++) sum += sums[j][tid];
-    a.out[(t.row0 + qi) * a.out_stride + (long)(hy / a.hgroups * a.group + hh) * HD + tid] =
-        L == 0.0f ? 0.0f : sum / (L * kWMul);
+  float4 o = make_float4(0, 0, 0, 0);
+  for (int s0 = 0; s0 < parts; s0 += kAhead * G) {
+    float4 u[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const int s = s0 + grp + (kAhead + j) * G;
+      u[j] = make_float4(0, 0, 0, 0);
+      if (grp < G && s < parts)
+        u[j] = *reinterpret_cast<const float4*>(part + (size_t)s * rows * HD);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const int s = s0 + grp + j * G;
+      const float f = W > 1 ? weight[s < kMaxParts ? s : 0] : __shfl(w[0], s & 63);
+      if (s < parts) {
+        o.x += f * v[j].x;
+        o.y += f * v[j].y;
+        o.z += f * v[j].z;
+        o.w += f * v[j].w;
+      }
+      v[j] = u[j];
+    }
+  }
+  float* dst = a.out + (long)(meta.x + qi) * a.out_stride + (long)(hy / a.hgroups * a.group + hh) * HD;
+  const float inv = L == 0.0f ? 0.0f : 1.0f / (L * kWMul);
+  if (W == 1) {
+    float4 r = o;
+#pragma unroll
+    for (int j = 1; j < G; j++) {
+      r.x += __shfl(o.x, tid + j * Q);
+      r.y += __shfl(o.y, tid + j * Q);
+      r.z += __shfl(o.z, tid + j * Q);
+      r.w += __shfl(o.w, tid + j * Q);
+    }
+    if (tid < Q)
+      *reinterpret_cast<float4*>(dst + 4 * c) =
+          make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
+  } else {
+    if (grp < G) *reinterpret_cast<float4*>(&sums[grp][4 * c]) = o;
+    __syncthreads();
+    if (tid < HD) {
+      float sum = 0.0f;
+      for (int j = 0; j < G; j++) sum += sums[j][tid];
+      dst[tid] = sum * inv;
+    }
   }
 }
 
@@ -619,8 +660,12 @@ void attn_launch(const AttnArgs& a, hipStream_t st) {
   if (a.rt == 1) hipLaunchKernelGGL((k_pool_attn<HD, 1>), grid, dim3(256), 0, st, a);
   if constexpr (HD <= 128)
     if (a.rt == 2) hipLaunchKernelGGL((k_pool_attn<HD, 2>), grid, dim3(256), 0, st, a);
-  if (a.splits > 1)
-    hipLaunchKernelGGL(k_pool_attn_join<HD>, dim3(16 * a.rt * a.slots, grid.y), dim3(256), 0, st, a);
+  if (a.splits > kJoinWave)
+    hipLaunchKernelGGL((k_pool_attn_join<HD, 4>), dim3(16 * a.rt * a.slots, grid.y), dim3(256), 0,
+                       st, a);
+  else if (a.splits > 1)
+    hipLaunchKernelGGL((k_pool_attn_join<HD, 1>), dim3(4 * a.rt * a.slots, grid.y), dim3(256), 0,
+                       st, a);
 }
 
 }  // namespace
@@ -628,7 +673,7 @@ void attn_launch(const AttnArgs& a, hipStream_t st) {
 size_t kv_attention_scratch(const PoolView& p, const Ragged& r, int n_heads, int max_len,
                             int window) {
   const AttnArgs a = attn_plan(p, r, n_heads, max_len, window);
-  return a.splits == 1 ? 0 : part_rows(a) * (p.hd + 2) * sizeof(float);
+  return a.splits == 1 ? 0 : part_rows(a) * (p.hd + 2) * sizeof(float) + a.slots * sizeof(int4);
 }
 
 hipError_t kv_attention_launch(const PoolView& p, const Ragged& r, int n_heads, const float* q,
@@ -642,6 +687,7 @@ hipError_t kv_attention_launch(const PoolView& p, const Ragged& r, int n_heads, 
   a.scale2 = scale * 1.44269504088896340736f;
   a.part = static_cast<float*>(work);
   a.ml = a.part + part_rows(a) * p.hd;
+  a.meta = reinterpret_cast<int4*>(a.ml + part_rows(a) * 2);
   switch (p.hd) {
     case 32: attn_launch<32>(a, st); break;
     case 64: attn_launch<64>(a, st); break;
