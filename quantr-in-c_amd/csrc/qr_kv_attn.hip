@@ -615,8 +615,12 @@ __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
 
 // How the work is cut.  Heads: at most 16 of a kv head's query heads share a
 // tile, as many queries beside each other as fill it; 32 rows where sequences bring
-// as many.  Tokens: a tile's part is one workgroup; there are as many parts as
-// it takes to have four workgroups per CU (lengths differ), each of a round or more.
+// as many.  Tokens: a tile's part is one workgroup.  The number of rounds of a part is the
+// one with the least time by what was measured (us): 3.5 before a workgroup's first
+// round and after its last, 0.4 + 0.009 head_dim a round, 5 for a thousand workgroups, 4 for
+// joining parts; 768 workgroups at once (512 where registers allow two a CU), of
+// several sequences 0.6 of the longest's parts filled.  (702 tokens of head_dim 64: one
+// part 8.2, three 10.4; 1500 of 128: one 14.2, six 11.0; 64 sequences of up to 1024: one 15.1, four 19.4.)
 AttnArgs attn_plan(const PoolView& p, const Ragged& r, int n_heads, int max_len, int window) {
   AttnArgs a = {};
   a.p = p;
@@ -637,13 +641,26 @@ AttnArgs attn_plan(const PoolView& p, const Ragged& r, int n_heads, int max_len,
   long range = max_len;
   if (window > 0 && window + (long)a.qpt + kStep < range) range = window + (long)a.qpt + kStep;
   const long tiles = (r.T / a.qpt > r.n ? r.T / a.qpt : r.n) * (long)p.n_kv_heads * a.hgroups;
-  long splits = tiles >= 384 ? 1 : (1024 + tiles - 1) / tiles;
+  const float at_once = a.rt == 1 && p.hd <= 128 ? 768.0f : 512.0f, filled = r.n > 1 ? 0.6f : 1.0f;
   const long most = (range + kRound - 1) / kRound;
-  if (splits > most) splits = most;
-  if (splits > kMaxParts) splits = kMaxParts;
-  if (splits < 1) splits = 1;
-  long chunk = (range + splits - 1) / splits;
-  chunk = (chunk + kStep - 1) / kStep * kStep;
+  float best = INFINITY;
+  long chunk = 0;
+  for (long rounds = 1;; rounds += 1 + rounds / 4) {
+    if (rounds > most) rounds = most;
+    const long parts = (most + rounds - 1) / rounds;
+    if (parts <= kMaxParts) {
+      const float wgs = (float)tiles * (float)parts;
+      const float turns = parts > 1 ? wgs * filled / at_once : wgs / at_once;
+      const float us = (turns > 1.0f ? turns : 1.0f) *
+                           (3.5f + (0.4f + 0.009f * (float)p.hd) * (float)rounds) +
+                       0.005f * wgs + (parts > 1 ? 4.0f : 0.0f);
+      if (us < best) {
+        best = us;
+        chunk = rounds * kRound;
+      }
+    }
+    if (rounds == most) break;
+  }
   a.chunk = (int)chunk;
   a.splits = (int)((range + chunk - 1) / chunk);
   return a;

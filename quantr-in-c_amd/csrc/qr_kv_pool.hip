@@ -620,8 +620,8 @@ int pool_check(const qr_ctx* c, const qr_kv_pool* p, const char* who) {
     return set_error(QR_ERR_INVALID, "%s: page %d (a power of two, 16 to 65536)", who, p->page);
   if (p->head_dim <= 0 || p->head_dim % 32 || p->head_dim > 256)
     return set_error(QR_ERR_INVALID, "%s: head_dim %d (a multiple of 32, <= 256)", who, p->head_dim);
-  if ((long)p->max_pages * p->page > 0x7FFFFF00l)
-    return set_error(QR_ERR_INVALID, "%s: %d pages of %d tokens exceed 2^31", who, p->max_pages,
+  if ((long)p->max_pages * p->page > 1l << 30)
+    return set_error(QR_ERR_INVALID, "%s: %d pages of %d tokens exceed 2^30", who, p->max_pages,
                      p->page);
   if (!p->data || !p->scale || !p->table || !p->len || !p->refs)
     return set_error(QR_ERR_INVALID, "%s: null pointer in the pool", who);
