@@ -71,8 +71,12 @@ struct CopyPlan {
 // ---- extend -----------------------------------------------------------------
 // One workgroup plans: which listed sequences copy their last page, how many
 // pages each takes (prefix sums), the free pages in order, and then writes the
-// tables.  It is bound by the latency of its few dependent steps; a larger
-// grid would have to agree on the plan first.
+// tables.  It is bound by the latency of its few dependent loads, so what does
+// not depend on others (the list, the first 4096 reference counts) is loaded at once,
+// and what is needed again stays in registers and LDS; a larger grid would have to
+// agree on the plan first.
+constexpr int kFirst = 4 * kPlan;   // pages whose reference counts are held in LDS
+constexpr int kFreeLds = 1536;      // free pages listed in LDS; more in scratch memory
 __global__ __launch_bounds__(kPlan) void k_pages_extend(PageState p, const int32_t* seqs,
                                                         const int32_t* add, int n, CopyPlan plan,
                                                         int32_t* freelist, int32_t* status) {
@@ -81,23 +85,39 @@ __global__ __launch_bounds__(kPlan) void k_pages_extend(PageState p, const int32
   __shared__ uint32_t seen[QR_KV_MAX_SEQS / 32];
   __shared__ int32_t last[QR_KV_MAX_LIST];   // the partly filled last page, -1: none
   __shared__ uint32_t off[QR_KV_MAX_LIST];   // first slot among the pages taken
-  __shared__ uint8_t cow[QR_KV_MAX_LIST];
+  __shared__ int32_t first[kFirst];          // reference counts
+  __shared__ int32_t freed[kFreeLds];
+  constexpr int kEach = QR_KV_MAX_LIST / kPlan;
   const int tid = threadIdx.x;
+  int s[kEach], more[kEach], len[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; j++) {
+    const int i = tid + j * kPlan;
+    s[j] = i < n ? seqs[i] : 0;
+    more[j] = i < n ? add[i] : 0;
+  }
+  const int4 head = refs4(p.refs, 4 * tid, p.n_pages, 1);
   for (int i = tid; i < (p.n_seqs + 31) / 32; i += kPlan) seen[i] = 0;
   if (tid == 0) bad = 0;
+  *reinterpret_cast<int4*>(&first[4 * tid]) = head;
+#pragma unroll
+  for (int j = 0; j < kEach; j++) {
+    const bool ok = (unsigned)s[j] < (unsigned)p.n_seqs;
+    len[j] = ok ? p.len[s[j]] : -1;
+  }
   __syncthreads();
-  for (int i = tid; i < n; i += kPlan) {
-    const int s = seqs[i], a = add[i];
+#pragma unroll
+  for (int j = 0; j < kEach; j++) {
+    const int i = tid + j * kPlan;
+    if (i >= n) continue;
     int l = -1;
-    if ((unsigned)s >= (unsigned)p.n_seqs || a < 0) {
+    const long L = len[j];
+    if (L < 0 || more[j] < 0 || L + more[j] > ((long)p.max_pages << p.page_shift)) {
       bad = 1;
     } else {
-      if (atomicOr(&seen[s >> 5], 1u << (s & 31)) & (1u << (s & 31))) bad = 1;
-      const long L = p.len[s];
-      if (L < 0 || L + a > ((long)p.max_pages << p.page_shift)) {
-        bad = 1;
-      } else if (a > 0 && (L & ((1l << p.page_shift) - 1))) {
-        l = p.table[(size_t)s * p.max_pages + (L >> p.page_shift)];
+      if (atomicOr(&seen[s[j] >> 5], 1u << (s[j] & 31)) & (1u << (s[j] & 31))) bad = 1;
+      if (more[j] > 0 && (L & ((1l << p.page_shift) - 1))) {
+        l = p.table[(size_t)s[j] * p.max_pages + (L >> p.page_shift)];
         if ((unsigned)l >= (unsigned)p.n_pages) bad = 1;
       }
     }
@@ -114,29 +134,31 @@ __global__ __launch_bounds__(kPlan) void k_pages_extend(PageState p, const int32
   // Of the listed sequences that share a last page, the earlier ones copy
   // while others still hold it.
   long base = 0, copies = 0;
-  for (int i0 = 0; i0 < n; i0 += kPlan) {
-    const int i = i0 + tid;
-    int c = 0;
+  int cow[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; j++) {
+    cow[j] = 0;
+    if (j * kPlan >= n) continue;  // the whole workgroup
+    const int i = tid + j * kPlan;
     long need = 0;
     if (i < n) {
       const int l = last[i];
       if (l >= 0) {
-        const int r = p.refs[l];
+        const int r = l < kFirst ? first[l] : p.refs[l];
         if (r > 1) {
           int before = 0;
-          for (int j = 0; j < i; j++) before += last[j] == l;
-          c = before < r - 1;
+          for (int k = 0; k < i; k++) before += last[k] == l;
+          cow[j] = before < r - 1;
         }
       }
-      const long L = p.len[seqs[i]];
-      need = c + pages_of(L + add[i], p.page_shift) - pages_of(L, p.page_shift);
-      cow[i] = (uint8_t)c;
+      need = cow[j] + pages_of((long)len[j] + more[j], p.page_shift) -
+             pages_of(len[j], p.page_shift);
     }
     long tot;
-    const long ex = block_scan((need << 16) + c, tmp, &tot);
+    const long ex = block_scan((need << 16) + cow[j], tmp, &tot);
     if (i < n) {
       off[i] = (uint32_t)(base + (ex >> 16));
-      if (c) {
+      if (cow[j]) {
         const long k = copies + (ex & 0xFFFF);
         plan.src[k] = last[i];
         plan.dst[k] = (int32_t)off[i];  // the slot, until the page is known
@@ -144,19 +166,19 @@ __global__ __launch_bounds__(kPlan) void k_pages_extend(PageState p, const int32
     }
     base += tot >> 16;
     copies += tot & 0xFFFF;
-    __syncthreads();
   }
   // the free pages in ascending order, as many as are taken
+  int32_t* const list = base <= kFreeLds ? freed : freelist;
   long found = 0;
   for (int i0 = 0; i0 < p.n_pages && found < base; i0 += 4 * kPlan) {
     const int i = i0 + 4 * tid;
-    const int4 r = refs4(p.refs, i, p.n_pages, 1);
+    const int4 r = i0 == 0 ? head : refs4(p.refs, i, p.n_pages, 1);
     const int f[4] = {r.x == 0, r.y == 0, r.z == 0, r.w == 0};
     long tot;
     long k = found + block_scan(f[0] + f[1] + f[2] + f[3], tmp, &tot);
     for (int j = 0; j < 4; j++)
       if (f[j]) {
-        if (k < base) freelist[k] = i + j;
+        if (k < base) list[k] = i + j;
         k++;
       }
     found += tot;
@@ -169,6 +191,21 @@ __global__ __launch_bounds__(kPlan) void k_pages_extend(PageState p, const int32
     }
     return;
   }
+  // each sequence's first page by its own thread, further ones by all
+#pragma unroll
+  for (int j = 0; j < kEach; j++) {
+    const int i = tid + j * kPlan;
+    if (i >= n) continue;
+    p.len[s[j]] = len[j] + more[j];
+    const long end = i + 1 < n ? (long)off[i + 1] : base;
+    if ((long)off[i] >= end) continue;
+    const int page = list[off[i]];
+    p.table[(size_t)s[j] * p.max_pages + pages_of(len[j], p.page_shift) - cow[j]] = page;
+    p.refs[page] = 1;
+    if (cow[j]) atomicAdd(&p.refs[last[i]], -1);
+    last[i] = pages_of(len[j], p.page_shift) - cow[j];  // where its pages begin
+  }
+  __syncthreads();
   for (long k = tid; k < base; k += kPlan) {
     int lo = 0, hi = n - 1;  // the last sequence whose first slot is not behind k
     while (lo < hi) {
@@ -178,18 +215,12 @@ __global__ __launch_bounds__(kPlan) void k_pages_extend(PageState p, const int32
       else
         hi = mid - 1;
     }
-    const int s = seqs[lo], rel = (int)(k - off[lo]), c = cow[lo];
-    const int have = pages_of(p.len[s], p.page_shift);
-    const int page = freelist[k];
-    p.table[(size_t)s * p.max_pages + have + rel - c] = page;
+    if ((long)off[lo] == k) continue;
+    const int page = list[k];
+    p.table[(size_t)seqs[lo] * p.max_pages + last[lo] + (int)(k - off[lo])] = page;
     p.refs[page] = 1;
   }
-  for (long k = tid; k < copies; k += kPlan) {
-    atomicAdd(&p.refs[plan.src[k]], -1);
-    plan.dst[k] = freelist[plan.dst[k]];
-  }
-  __syncthreads();
-  for (int i = tid; i < n; i += kPlan) p.len[seqs[i]] += add[i];
+  for (long k = tid; k < copies; k += kPlan) plan.dst[k] = list[plan.dst[k]];
   if (tid == 0) {
     plan.count[0] = (int32_t)copies;
     if (status) status[0] = QR_OK;

@@ -142,6 +142,20 @@ def test_many_sequences_in_one_list(dev):
     R.assert_same(d, p)
 
 
+def test_large_extends(dev):
+    """More free pages than fit the plan's LDS, reference counts beyond it."""
+    p = R.Pool(1, 9000, 16, 1, 32, 5, 3000, 1)
+    d = R.DevPool(dev, p)
+    for seqs, add in (([3], [40000]), ([0, 1], [1, 16 * 2100 + 5]), ([4, 3, 0], [17, 3, 40]),
+                      ([2], [16 * 2999]), ([2], [16 * 1700])):
+        assert p.extend(seqs, add) == d.extend(seqs, add)
+        R.assert_same(d, p, str(seqs))
+    assert p.trim([3, 1], [900, 16 * 1500]) == d.trim([3, 1], [900, 16 * 1500])
+    assert p.assign([2, 4], [1, 0]) == d.assign([2, 4], [1, 0]) == 0
+    assert p.extend([2, 1, 4], [9, 9, 1]) == d.extend([2, 1, 4], [9, 9, 1])
+    R.assert_same(d, p)
+
+
 def test_reset_and_optional_outputs(dev):
     p = filled(9, [37, 5], page=32)
     d = R.DevPool(dev, p)
@@ -324,6 +338,15 @@ def test_attention_of_long_sequences_in_parts(dev):
     check(d, p, [2, 0], [1, 3], 16, 2, max_len=3001, window=700, layer=1)
     again = check(d, p, [0, 1, 2], [1, 1, 1], 16, 1, max_len=3001, layer=1)
     np.testing.assert_array_equal(a.view(np.uint32), again.view(np.uint32))
+
+
+def test_attention_of_more_rounds_than_pages_are_held(dev):
+    """A part of over 16384 tokens (the bound on the lengths is far too small),
+    alone and behind a window."""
+    p = filled(36, [17001, 40], page=16, kv_heads=1, hd=32)
+    d = R.DevPool(dev, p)
+    check(d, p, [0, 1], [1, 1], 2, 1, max_len=64)
+    check(d, p, [1, 0], [2, 3], 2, 2, max_len=64, window=16900)
 
 
 def test_attention_of_peaked_and_flat_scores(dev):
