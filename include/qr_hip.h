@@ -527,7 +527,7 @@ int qr_kv_pool_attention(qr_ctx* ctx, const qr_kv_pool* pool, int layer, const i
  * = the number of logits ahead of the target's (greater ones, and equal ones
  * of lower index); top_id / top_lp [r][n_top], n_top <= QR_LOGPROBS_MAX_TOP: the most
  * probable tokens, equal ones by ascending index, with their log
- * probabilities (id -1 and -inf behind the vocabulary).  Each output may be
+ * probabilities (id -1 and -inf behind the vocabulary).  rows <= 2^23, vocab <= 2^30.  Each output may be
  * null; targets may be null where lp and rank are.  A target outside the
  * vocabulary gives lp 0 and rank -1.  Logits of -inf have probability 0; a row
  * of nothing else gives lp -inf, entropy 0.  A row that holds a NaN or +inf

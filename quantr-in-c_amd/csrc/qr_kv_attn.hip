@@ -28,9 +28,10 @@
 // times as many sums, held 206 registers for 168, and ended in a join of the waves.
 //
 // The weights carry V's scale: with vs = f 2^e (1 <= f < 2), w_t = f 2^(s_t
-// log2(e) + e - M) against the running maximum M of the exponents, so the
-// digits are taken from the numbers that are summed; the denominator adds the
-// same powers times 2^-e.  Both are exact but for exp2.
+// log2(e) + e - M) against the running maximum M of these exponents, so the
+// digits are taken from the numbers that are summed.  The denominator runs
+// against the maximum N of the scores alone, its terms the same powers times 2^(M - e
+// - N): values of V however unlike move no token out of it.
 #include <math.h>
 
 #include "qr_kv_pool.h"
@@ -54,8 +55,11 @@ constexpr float kWMul = 4177800.0f;
 constexpr float kWAdd = 8388608.0f + 32896.0f;
 constexpr float kQMax = 8355711.0f;  // 127 * (65536 + 256 + 1)
 // Exponent of V scales that are 0 or smaller than it: such a block's weights
-// lead no others, and its tokens still count in the denominator (at 2^60).
+// lead no others.
 constexpr int kMinExp = -60;
+// A block whose exponents lie further below M takes its powers 2^-kDeep below them, so that
+// they are there for the denominator.
+constexpr float kDeep = 60.0f;
 
 // Where the rows of tile `slot` come from.
 struct Tile {
@@ -78,7 +82,7 @@ struct AttnArgs {
   int chunk;            // tokens of a part, a multiple of kStep
   int window;
   float scale2;         // scale * log2(e)
-  float* part;          // [tile, head][splits][row][hd], then [..][row][2]
+  float* part;          // [tile, head][splits][row][hd], then [..][row][4]
   float* ml;
   int4* meta;           // [tile]: first row, queries, parts
 };
@@ -168,15 +172,21 @@ __device__ inline float lift(float m, float to) {
   return m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
 }
 
+// What a sum against M is multiplied by for the result, with the denominator l
+// against N; 0 for a row that saw nothing.
+__device__ inline float over(float M, float N, float l) {
+  return l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(M - N) / (l * kWMul);
+}
+
 template <int HD, int RT>
 __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) void k_pool_attn(AttnArgs a) {
   constexpr int NC = (HD + 63) / 64;            // 64-column chunks of a K row
   constexpr int NV = (HD / 16 + 3) / kWaves;    // 16-column tiles of V for a wave
   __shared__ int4 sp[kWaves][RT][3][64];        // the weights' digits
-  __shared__ int8_t sq[3][16 * RT][NC * 64 + 16];  // the rows' digits
+  __shared__ __align__(16) int8_t sq[3][16 * RT][NC * 64 + 16];  // the rows' digits
   __shared__ float sqs[16 * RT];                   // and what one of the last place stands for
   __shared__ int spg[kPages];
-  __shared__ float smax[kWaves][RT][16];
+  __shared__ float smax[kWaves][RT][16], smaxs[kWaves][RT][16];
   __shared__ float ssum[kWaves][RT][16];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -299,7 +309,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
       amax = fmaxf(amax, __shfl_xor(amax, d));
       bad = fmaxf(bad, __shfl_xor(bad, d));
     }
-    // below 2^-96 a row's scores are 0 beside any scale of K that fp32 values give
+    // a row below 2^-96 is held to 2^-119
     amax = fmaxf(amax, 1.2621774e-29f);
     const float inv = kQMax / amax;
     uint32_t u[4];
@@ -320,10 +330,10 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
 #pragma unroll
   for (int r = 0; r < RT; r++) qs[r] = sqs[16 * r + n];
 
-  float o[RT][NV][4], M[RT], L[RT];
+  float o[RT][NV][4], M[RT], N[RT], L[RT];
 #pragma unroll
   for (int r = 0; r < RT; r++) {
-    M[r] = kNone;
+    M[r] = N[r] = kNone;
     L[r] = 0.0f;
 #pragma unroll
     for (int d = 0; d < NV; d++)
@@ -334,8 +344,8 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
   for (int T0 = tb; T0 < te; T0 += kRound) {
     const int Tw = T0 + wave * kStep;  // of the wave
     const bool mine = Tw < te;
-    float e[RT][16], mx[RT];
-    float back = 0.0f, fw = 0.0f;
+    float e[RT][16], mx[RT];  // exponents, and their largest of the lane's block
+    float evf = 0.0f, fw = 0.0f;
 #pragma unroll
     for (int r = 0; r < RT; r++) mx[r] = kNone;
     if (mine) {
@@ -343,9 +353,8 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
       const float vs = sc.y;
       int ev = kMinExp;
       if (vs > 0x1p-60f) ev = (int)((__builtin_bit_cast(uint32_t, vs) >> 23) & 255) - 127;
-      back = __builtin_bit_cast(float, (uint32_t)(127 - ev) << 23);
-      fw = vs * back * kWMul;
-      const float evf = (float)ev;
+      fw = vs * __builtin_bit_cast(float, (uint32_t)(127 - ev) << 23) * kWMul;
+      evf = (float)ev;
       // Every token of the step seen by every row of the tile?
       const bool full = __all(here) && Tw + kStep <= t.pos0 + 1 &&
                         (a.window == 0 || Tw >= t.pos0 + t.queries - a.window);
@@ -380,12 +389,16 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
         }
 #pragma unroll
         for (int j = 0; j < 16; j++) mx[r] = fmaxf(mx[r], e[r][j]);
-        mx[r] = rows_max(mx[r]);
       }
     }
-    if (g == 0)
 #pragma unroll
-      for (int r = 0; r < RT; r++) smax[wave][r][n] = mx[r];
+    for (int r = 0; r < RT; r++) {
+      const float m = rows_max(mx[r]), s = rows_max(mx[r] - evf);
+      if (g == 0) {
+        smax[wave][r][n] = m;
+        smaxs[wave][r][n] = s;
+      }
+    }
     // This round's V, and behind it the next one's K.
     load_v(T0);
     const int Tn = T0 + kRound;
@@ -409,10 +422,17 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     for (int r = 0; r < RT; r++) {
       const float to = fmaxf(M[r], fmaxf(fmaxf(smax[0][r][n], smax[1][r][n]),
                                          fmaxf(smax[2][r][n], smax[3][r][n])));
-      const float ref = to == kNone ? 0.0f : to;
+      const float tos = fmaxf(N[r], fmaxf(fmaxf(smaxs[0][r][n], smaxs[1][r][n]),
+                                          fmaxf(smaxs[2][r][n], smaxs[3][r][n])));
+      const float ref = to == kNone ? 0.0f : to, refs = tos == kNone ? 0.0f : tos;
       alpha[r] = lift(M[r], ref);
+      L[r] *= lift(N[r], refs);
       M[r] = to;
+      N[r] = tos;
       if (mine) {
+        // 0 but for blocks far below M (and 300 for those that nothing is seen of)
+        const float deep = fminf(fmaxf(ceilf(ref - mx[r]) - kDeep, 0.0f), 300.0f);
+        const float base = ref - deep, fwd = __builtin_ldexpf(fw, -(int)deep);
         float sum = 0.0f;
         int4 p[3];
         int* d0 = &p[0].x;
@@ -423,18 +443,17 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
           uint32_t u[4];
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const float w = __builtin_amdgcn_exp2f(e[r][4 * tt + i] - ref);
+            const float w = __builtin_amdgcn_exp2f(e[r][4 * tt + i] - base);
             sum += w;
-            u[i] = __builtin_bit_cast(uint32_t, __builtin_fmaf(w, fw, kWAdd));
+            u[i] = __builtin_bit_cast(uint32_t, __builtin_fmaf(w, fwd, kWAdd));
           }
           digits4(u[0], u[1], u[2], u[3], d0 + tt, d1 + tt, d2 + tt);
         }
-        L[r] = __builtin_fmaf(sum, back, L[r] * alpha[r]);
+        L[r] = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(base - evf - refs), L[r]);
 #pragma unroll
         for (int k = 0; k < 3; k++) sp[wave][r][k][lane] = p[k];
       } else {
         // no tokens: digits of 0, whatever V holds there
-        L[r] *= alpha[r];
 #pragma unroll
         for (int k = 0; k < 3; k++) sp[wave][r][k][lane] = make_int4(0, 0, 0, 0);
       }
@@ -480,7 +499,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     if (!row_ok[r]) continue;
     const float l = (ssum[0][r][n] + ssum[1][r][n]) + (ssum[2][r][n] + ssum[3][r][n]);
     if (a.splits == 1) {
-      const float inv = l == 0.0f ? 0.0f : 1.0f / (l * kWMul);  // 0: a row that saw nothing
+      const float inv = over(M[r], N[r], l);
       float* dst = a.out + row[r] * a.out_stride + (long)head[r] * HD + 4 * g;
 #pragma unroll
       for (int d = 0; d < NV; d++)
@@ -496,7 +515,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
           *reinterpret_cast<float4*>(a.part + at * HD + 16 * (wave + 4 * d) + 4 * g) =
               make_float4(o[r][d][0], o[r][d][1], o[r][d][2], o[r][d][3]);
       if (wave == 0 && g == 0)
-        *reinterpret_cast<float2*>(a.ml + 2 * at) = make_float2(M[r], l);
+        *reinterpret_cast<float4*>(a.ml + 4 * at) = make_float4(M[r], N[r], l, 0.0f);
     }
   }
 }
@@ -510,21 +529,22 @@ __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
   constexpr int Q = HD / 4, G = 64 * W / Q;  // threads of a part's columns, parts side by side
   constexpr int kEach = W == 1 ? 1 : kMaxParts / 256, kAhead = W == 1 ? 8 : 4;
   __shared__ float weight[W == 1 ? 1 : kMaxParts];
-  __shared__ float red[8];
-  __shared__ float sums[W == 1 ? 1 : G][HD];
+  __shared__ float red[12];
+  __shared__ __align__(16) float sums[W == 1 ? 1 : G][HD];
   const int rows = 16 * a.rt, tid = threadIdx.x % (64 * W);
   const int item = blockIdx.x * (4 / W) + threadIdx.x / (64 * W);
   const int n = item % rows, slot = item / rows, hy = blockIdx.y;
   const size_t at = (size_t)(slot * gridDim.y + hy) * a.splits * rows + n;
   const int4 meta = a.meta[slot];
-  float m[kEach], l[kEach];
+  float m[kEach], ns[kEach], l[kEach];
 #pragma unroll
   for (int j = 0; j < kEach; j++) {
     const int s = tid + 256 * j;
-    float2 v = make_float2(kNone, 0.0f);
-    if (s < a.splits) v = *reinterpret_cast<const float2*>(a.ml + 2 * (at + (size_t)s * rows));
+    float4 v = make_float4(kNone, kNone, 0.0f, 0.0f);
+    if (s < a.splits) v = *reinterpret_cast<const float4*>(a.ml + 4 * (at + (size_t)s * rows));
     m[j] = v.x;
-    l[j] = v.y;
+    ns[j] = v.y;
+    l[j] = v.z;
   }
   const int c = tid % Q, grp = tid / Q;
   const float* part = a.part + at * HD + 4 * c;
@@ -539,25 +559,36 @@ __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
   const int qi = n / a.hpt, hh = hy % a.hgroups * a.hpt + n % a.hpt;
   if (!(qi < meta.y && hh < a.group)) return;
   const int parts = meta.z < a.splits ? meta.z : a.splits;
-  float M = kNone, L = 0.0f;
+  float M = kNone, N = kNone, L = 0.0f;
 #pragma unroll
   for (int j = 0; j < kEach; j++) {
-    if (tid + 256 * j >= parts) m[j] = kNone;  // a part that is not there holds anything
+    if (tid + 256 * j >= parts) {  // a part that is not there holds anything
+      m[j] = ns[j] = kNone;
+      l[j] = 0.0f;
+    }
     M = fmaxf(M, m[j]);
+    N = fmaxf(N, ns[j]);
   }
-  for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
+  for (int d = 32; d; d >>= 1) {
+    M = fmaxf(M, __shfl_xor(M, d));
+    N = fmaxf(N, __shfl_xor(N, d));
+  }
   if (W > 1) {
-    if ((tid & 63) == 0) red[tid >> 6] = M;
+    if ((tid & 63) == 0) {
+      red[tid >> 6] = M;
+      red[8 + (tid >> 6)] = N;
+    }
     __syncthreads();
     M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    N = fmaxf(fmaxf(red[8], red[9]), fmaxf(red[10], red[11]));
   }
-  const float ref = M == kNone ? 0.0f : M;
+  const float ref = M == kNone ? 0.0f : M, refs = N == kNone ? 0.0f : N;
   float w[kEach];
 #pragma unroll
   for (int j = 0; j < kEach; j++) {
     w[j] = lift(m[j], ref);
     if (W > 1) weight[tid + 256 * j] = w[j];
-    if (m[j] != kNone) L += w[j] * l[j];
+    L += lift(ns[j], refs) * l[j];
   }
   for (int d = 32; d; d >>= 1) L += __shfl_xor(L, d);
   if (W > 1) {
@@ -589,7 +620,7 @@ __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
     }
   }
   float* dst = a.out + (long)(meta.x + qi) * a.out_stride + (long)(hy / a.hgroups * a.group + hh) * HD;
-  const float inv = L == 0.0f ? 0.0f : 1.0f / (L * kWMul);
+  const float inv = over(M, N, L);
   if (W == 1) {
     float4 r = o;
 #pragma unroll
@@ -690,7 +721,7 @@ void attn_launch(const AttnArgs& a, hipStream_t st) {
 size_t kv_attention_scratch(const PoolView& p, const Ragged& r, int n_heads, int max_len,
                             int window) {
   const AttnArgs a = attn_plan(p, r, n_heads, max_len, window);
-  return a.splits == 1 ? 0 : part_rows(a) * (p.hd + 2) * sizeof(float) + a.slots * sizeof(int4);
+  return a.splits == 1 ? 0 : part_rows(a) * (p.hd + 4) * sizeof(float) + a.slots * sizeof(int4);
 }
 
 hipError_t kv_attention_launch(const PoolView& p, const Ragged& r, int n_heads, const float* q,
@@ -704,7 +735,7 @@ hipError_t kv_attention_launch(const PoolView& p, const Ragged& r, int n_heads, 
   a.scale2 = scale * 1.44269504088896340736f;
   a.part = static_cast<float*>(work);
   a.ml = a.part + part_rows(a) * p.hd;
-  a.meta = reinterpret_cast<int4*>(a.ml + part_rows(a) * 2);
+  a.meta = reinterpret_cast<int4*>(a.ml + part_rows(a) * 4);
   switch (p.hd) {
     case 32: attn_launch<32>(a, st); break;
     case 64: attn_launch<64>(a, st); break;

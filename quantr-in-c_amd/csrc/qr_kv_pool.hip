@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kPlan) void k_pages_extend(PageState p, const int32
   __shared__ uint32_t seen[QR_KV_MAX_SEQS / 32];
   __shared__ int32_t last[QR_KV_MAX_LIST];   // the partly filled last page, -1: none
   __shared__ uint32_t off[QR_KV_MAX_LIST];   // first slot among the pages taken
-  __shared__ int32_t first[kFirst];          // reference counts
+  __shared__ __align__(16) int32_t first[kFirst];  // reference counts
   __shared__ int32_t freed[kFreeLds];
   constexpr int kEach = QR_KV_MAX_LIST / kPlan;
   const int tid = threadIdx.x;

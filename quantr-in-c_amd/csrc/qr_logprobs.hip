@@ -597,7 +597,7 @@ extern "C" int qr_logprobs(qr_ctx* c, const float* x, long stride, int rows, int
                            int n_top, int32_t* top_id, float* top_lp) {
   const char* who = "qr_logprobs";
   if (!c) return set_error(QR_ERR_INVALID, "%s: null ctx", who);
-  if (rows < 0 || vocab <= 0 || stride < vocab)
+  if (rows < 0 || rows > 1 << 23 || vocab <= 0 || vocab > 1 << 30 || stride < vocab)
     return set_error(QR_ERR_INVALID, "%s: %d rows of %d logits, stride %ld", who, rows, vocab,
                      stride);
   if (n_top < 0 || n_top > QR_LOGPROBS_MAX_TOP)

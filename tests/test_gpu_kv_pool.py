@@ -349,6 +349,29 @@ def test_attention_of_more_rounds_than_pages_are_held(dev):
     check(d, p, [1, 0], [2, 3], 2, 2, max_len=64, window=16900)
 
 
+def test_rows_before_the_first_sequence(dev):
+    """start[0] > 0: rows of nobody before the first sequence stay, others are found."""
+    p = filled(37, [50, 7, 90], page=32, kv_heads=2, hd=64)
+    d = R.DevPool(dev, p)
+    rng = np.random.default_rng(5)
+    for st in ([5, 6, 7, 8], [21, 23, 23, 40], [3, 3, 3, 4]):
+        st = np.array(st, np.int32)
+        q = rng.normal(0, 1, (45, 4 * 64)).astype(np.float32)
+        got = d.attention(0, [0, 1, 2], st, q, 4)
+        want = p.attention(0, [0, 1, 2], st, q, 4)
+        bound = R.attention_bound(p, 0, [0, 1, 2], st, q, 4)
+        own = slice(st[0], st[-1])
+        assert (np.abs(got[own] - want[own]) <= bound[own]).all()
+        assert (got[:st[0]] == 7).all() and (got[st[-1]:] == 7).all()
+        k = rng.normal(0, 1, (45, 128)).astype(np.float32)
+        p.store(0, [0, 1, 2], st, k, -k)
+        d.store(0, [0, 1, 2], st, k, -k)
+        R.assert_same(d, p)
+        back = d.load(0, [0, 1, 2], st, 45)
+        for x in back:
+            assert (x[:st[0]] == 7).all() and (x[st[-1]:] == 7).all()
+
+
 def test_attention_of_peaked_and_flat_scores(dev):
     p = filled(32, [500, 333], page=32, kv_heads=2, hd=128)
     d = R.DevPool(dev, p)
@@ -370,6 +393,16 @@ def test_attention_of_unlike_blocks(dev):
     d = R.DevPool(dev, p)
     check(d, p, [0], [1], 4, 1)
     check(d, p, [0], [33], 4, 2)
+    # tiny or no values before, beside and behind ones near the largest float
+    for scales in ((0.0, 1e36, 1e-3, 0.0) * 3 + (0.0,), (1e36,) * 2 + (1e-36,) * 11,
+                   (1e-38,) * 9 + (1e30,) * 4, (1e-44, 1e36) * 6 + (1e-44,)):
+        for b, s in enumerate(scales):
+            g, bb = p.table[0, b * 16 // 32], b % 2
+            p.scale[0, g, 0, bb, 1] = s
+        p.data[:] = d0
+        d = R.DevPool(dev, p)
+        check(d, p, [0], [1], 4, 3)
+        check(d, p, [0], [40], 4, 4)
     for b in range(13):  # and nothing but zeros
         g, bb = p.table[0, b * 16 // 32], b % 2
         p.scale[0, g, 0, bb] = 0
