@@ -35,6 +35,7 @@
 #include <math.h>
 
 #include "qr_kv_pool.h"
+#include "qr_lanes.h"
 
 namespace qr {
 namespace {
@@ -87,18 +88,21 @@ struct AttnArgs {
   int4* meta;           // [tile]: first row, queries, parts
 };
 
-__device__ inline Tile tile_of(const AttnArgs& a, int slot) {
+// All but its length and positions, which tile_len adds.
+__device__ inline Tile tile_of(const AttnArgs& a, int slot, SeqRows* s) {
   Tile t;
   int piece;
-  const SeqRows s = slot_rows(a.p, a.r, slot, a.qpt, a.extra, &piece);
+  *s = slot_rows(a.p, a.r, slot, a.qpt, a.extra, &piece);
   const int at = piece * a.qpt;
-  t.row0 = s.row0 + at;
-  t.queries = s.m - at < a.qpt ? s.m - at : a.qpt;
-  if (piece < 0 || at >= s.m) t.queries = 0;
-  t.seq = s.seq;
-  t.len = s.len;
-  t.pos0 = s.len - s.m + at;
+  t.row0 = s->row0 + at;
+  t.queries = s->m - at < a.qpt ? s->m - at : a.qpt;
+  if (piece < 0 || at >= s->m) t.queries = 0;
+  t.seq = s->seq;
   return t;
+}
+__device__ inline void tile_len(const AttnArgs& a, const SeqRows& s, Tile* t) {
+  t->len = seq_len(a.p, s);
+  t->pos0 = t->len - s.m + (t->row0 - s.row0);
 }
 
 // Which tile and part a workgroup takes.  The last tiles, whose rows see most, come
@@ -154,16 +158,6 @@ __device__ inline float joined(int s2, int s1, int s0) {
   return __builtin_fmaf((float)(s2 * 256 + s1), 256.0f, (float)s0);
 }
 
-// Over the four lane groups of a row.
-__device__ inline float rows_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
-}
-__device__ inline float rows_sum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
-}
-
 __device__ inline int4 load16(const int8_t* p) { return *reinterpret_cast<const int4*>(p); }
 __device__ inline v4i as_v4(int4 x) { return v4i{x.x, x.y, x.z, x.w}; }
 
@@ -195,18 +189,38 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
   work_of(a, &slot, &z);
   const int hy = blockIdx.y;
   const int kvh = hy / a.hgroups, hg = hy % a.hgroups;
-  const Tile t = tile_of(a, slot);
-  // Pages of a round's 16 blocks, one in each lane group's lanes; -1: none.
+  SeqRows seq;
+  Tile t = tile_of(a, slot, &seq);
+  if (t.queries == 0) {
+    if (a.splits > 1 && z == 0 && hy == 0 && threadIdx.x == 0) a.meta[slot] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  // What hangs on the sequence alone is fetched together: the first round's pages where no window
+  // moves it (one of its 16 blocks in each lane group's lanes; -1: none), q, the length.
   auto pages = [&](int T0) { return page_at(a.p, t.seq, (T0 + 16 * n) >> a.p.page_shift); };
-  // The first round's, where no window moves it, before the length is there.
   int pg = -1;
   if (a.window == 0) pg = pages(z * a.chunk);
+  // q: kPer lanes share a row, four columns each; a wave takes every fourth set of rows.
+  constexpr int kPer = NC == 1 ? 16 : NC == 2 ? 32 : 64, kSets = 64 / kPer;
+  constexpr int kTurns = 16 * RT / (kWaves * kSets);
+  const int qc = lane % kPer * 4;
+  float4 x[kTurns];
+#pragma unroll
+  for (int i = 0; i < kTurns; i++) {
+    const int at = (i * kWaves + wave) * kSets + lane / kPer;
+    const int qi = at / a.hpt, hh = hg * a.hpt + at % a.hpt;
+    x[i] = make_float4(0, 0, 0, 0);
+    if (qi < t.queries && hh < a.group && qc < HD)
+      x[i] = *reinterpret_cast<const float4*>(a.q + (t.row0 + qi) * a.q_stride +
+                                              (long)(kvh * a.group + hh) * HD + qc);
+  }
+  tile_len(a, seq, &t);
   int lo, hi, tb, te;
   tile_range(a, t, &lo, &hi);
   part_range(a, lo, hi, z, &tb, &te);
   if (a.splits > 1 && z == 0 && hy == 0 && threadIdx.x == 0)  // for the joining launch
     a.meta[slot] = make_int4(t.row0, t.queries, hi > lo ? (hi - lo - 1) / a.chunk + 1 : 0, 0);
-  if (t.queries == 0 || (tb >= te && a.splits > 1)) return;
+  if (tb >= te && a.splits > 1) return;
   if (a.window > 0) pg = pages(tb);
   if (tb + 16 * n >= te) pg = -1;
   // Those of later rounds by way of LDS, kPages blocks at a time: a load of them in the
@@ -234,21 +248,6 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     // positions before 0 see nothing
     row_hi[r] = row_ok[r] && t.pos0 + qi >= 0 ? t.pos0 + qi + 1 : 0;
     row_lo[r] = a.window > 0 ? row_hi[r] - a.window : 0;
-  }
-
-  // q: kPer lanes share a row, four columns each; a wave takes every fourth set of rows.
-  constexpr int kPer = NC == 1 ? 16 : NC == 2 ? 32 : 64, kSets = 64 / kPer;
-  constexpr int kTurns = 16 * RT / (kWaves * kSets);
-  const int qc = lane % kPer * 4;
-  float4 x[kTurns];
-#pragma unroll
-  for (int i = 0; i < kTurns; i++) {
-    const int at = (i * kWaves + wave) * kSets + lane / kPer;
-    const int qi = at / a.hpt, hh = hg * a.hpt + at % a.hpt;
-    x[i] = make_float4(0, 0, 0, 0);
-    if (qi < t.queries && hh < a.group && qc < HD)
-      x[i] = *reinterpret_cast<const float4*>(a.q + (t.row0 + qi) * a.q_stride +
-                                              (long)(kvh * a.group + hh) * HD + qc);
   }
 
   // K of the wave's step, its blocks' scales, and V's columns of the round
@@ -304,10 +303,15 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
       amax = fmaxf(amax, f);
       bad = f <= 3.402823466e+38f ? bad : 1.0f;
     }
-#pragma unroll
-    for (int d = 1; d < kPer; d <<= 1) {
-      amax = fmaxf(amax, __shfl_xor(amax, d));
-      bad = fmaxf(bad, __shfl_xor(bad, d));
+    amax = row_max(amax);
+    bad = row_max(bad);
+    if (kPer >= 32) {
+      amax = fmaxf(amax, lane_xor_f<16>(amax));
+      bad = fmaxf(bad, lane_xor_f<16>(bad));
+    }
+    if (kPer == 64) {
+      amax = fmaxf(amax, lane_xor_f<32>(amax));
+      bad = fmaxf(bad, lane_xor_f<32>(bad));
     }
     // a row below 2^-96 is held to 2^-119
     amax = fmaxf(amax, 1.2621774e-29f);
@@ -569,10 +573,8 @@ __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
     M = fmaxf(M, m[j]);
     N = fmaxf(N, ns[j]);
   }
-  for (int d = 32; d; d >>= 1) {
-    M = fmaxf(M, __shfl_xor(M, d));
-    N = fmaxf(N, __shfl_xor(N, d));
-  }
+  M = wave_max(M);
+  N = wave_max(N);
   if (W > 1) {
     if ((tid & 63) == 0) {
       red[tid >> 6] = M;
@@ -590,7 +592,7 @@ __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
     if (W > 1) weight[tid + 256 * j] = w[j];
     L += lift(ns[j], refs) * l[j];
   }
-  for (int d = 32; d; d >>= 1) L += __shfl_xor(L, d);
+  L = wave_sum(L);
   if (W > 1) {
     if ((tid & 63) == 0) red[4 + (tid >> 6)] = L;
     __syncthreads();

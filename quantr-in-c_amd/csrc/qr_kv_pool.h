@@ -40,18 +40,25 @@ __device__ inline int ragged_start(const Ragged& r, int i) {
   return s < 0 ? 0 : s > r.T ? r.T : s;
 }
 
-// A sequence of the batch: its row of the table, its rows and its length (0
-// where that row of the table does not exist).
+// A sequence of the batch: its row of the table (0 and not `there` where it does not
+// exist), its rows and its length.
 struct SeqRows {
   int seq, row0, m, len;
+  bool there;
 };
+__device__ inline int seq_len(const PoolView& p, const SeqRows& s) {
+  const long cap = (long)p.max_pages << p.page_shift;
+  const int n = p.len[s.seq];
+  return !s.there || n < 0 ? 0 : n > cap ? (int)cap : n;
+}
 
 // Which sequence a slot serves, where each sequence's rows are cut into pieces
 // of q rows: sequence i has the slots from start[i] / q + extra * i on.  There
 // are never fewer than its pieces (floor(b / q) - floor(a / q) + 1 >=
 // ceil((b - a) / q)), so the host sizes the grid by T / q + extra * n without
 // knowing the lengths, and a slot without a piece ends.  *piece: which of the
-// sequence's slots this is, < 0 for none.
+// sequence's slots this is, < 0 for none.  The length is not looked up here: other loads go
+// out beside it (seq_len).
 //
 // All lanes of the wave search at once, 64 places a step, and what is needed of
 // the place is loaded beside it: up to 64 sequences take two dependent
@@ -82,14 +89,9 @@ __device__ inline SeqRows slot_rows(const PoolView& p, const Ragged& r, int slot
       if (s.m < 0) s.m = 0;
       s.seq = __builtin_amdgcn_readlane(seq, k);
       *piece = slot - (s.row0 / q + extra * (lo + k));
+      s.there = (unsigned)s.seq < (unsigned)p.n_seqs;
+      if (!s.there) s.seq = 0;
       s.len = 0;
-      if ((unsigned)s.seq >= (unsigned)p.n_seqs) {
-        s.seq = 0;
-        return s;
-      }
-      const long cap = (long)p.max_pages << p.page_shift;
-      const int n = p.len[s.seq];
-      s.len = n < 0 ? 0 : n > cap ? (int)cap : n;
       return s;
     }
     lo += k * step;

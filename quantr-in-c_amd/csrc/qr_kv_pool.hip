@@ -11,6 +11,7 @@
 #include <math.h>
 
 #include "qr_kv_pool.h"
+#include "qr_lanes.h"
 
 namespace qr {
 namespace {
@@ -441,6 +442,7 @@ __device__ inline BlockRows block_rows(const PoolView& p, const Ragged& r, int s
   BlockRows b;
   b.any = b.there = false;
   b.s = slot_rows(p, r, slot, kKvBlock, 2, &b.piece);
+  b.s.len = seq_len(p, b.s);
   if (b.piece < 0 || b.s.m == 0) return b;
   const int pos0 = b.s.len - b.s.m;  // of the first row; < 0 where there are more rows than tokens
   const long lb = (long)(pos0 < 0 ? 0 : pos0) / kKvBlock + b.piece;
@@ -452,11 +454,6 @@ __device__ inline BlockRows block_rows(const PoolView& p, const Ragged& r, int s
   b.there = true;
   b.blk = block_at(p, page, kvh, (int)lb & ((1 << (p.page_shift - 4)) - 1));
   return b;
-}
-
-__device__ inline float wave_max(float v) {
-  for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-  return v;
 }
 
 // x / s rounded to the nearest even integer, for a normal s and |x| <= 127 s

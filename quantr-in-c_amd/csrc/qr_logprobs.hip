@@ -14,6 +14,7 @@
 #include <math.h>
 
 #include "qr_internal.h"
+#include "qr_lanes.h"
 
 namespace qr {
 namespace {
@@ -68,62 +69,19 @@ __device__ inline Sums join(const Sums& a, const Sums& b) {
   return r;
 }
 
-// The value of the lane whose number differs by the bits of X, without LDS (by way of
-// which a sort takes half as long again): 1, 2, 3 within a quad, 7 and 15 mirrored halves
-// of a row and rows, 8 a row turned by half, 16 and 32 by swapping rows.
-template <int X>
-__device__ inline uint32_t lane_xor(uint32_t v) {
-  constexpr int kCtrl = X == 1 ? 0xB1 : X == 2 ? 0x4E : X == 3 ? 0x1B : X == 7 ? 0x141
-                      : X == 15 ? 0x140 : 0x128;
-  if constexpr (X == 4) {
-    return lane_xor<3>(lane_xor<7>(v));
-  } else if constexpr (X == 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return threadIdx.x & 16 ? r[0] : r[1];
-  } else if constexpr (X == 32) {
-    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return threadIdx.x & 32 ? r[0] : r[1];
-  } else if constexpr (X == 31) {
-    return lane_xor<15>(lane_xor<16>(v));
-  } else if constexpr (X == 63) {
-    return lane_xor<31>(lane_xor<32>(v));
-  } else {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xF, 0xF, true);
-  }
-}
-template <int X>
-__device__ inline float lane_xor_f(float v) {
-  return __builtin_bit_cast(float, lane_xor<X>(__builtin_bit_cast(uint32_t, v)));
-}
-template <int X>
-__device__ inline u64 lane_xor_64(u64 k) {
-  return (u64)lane_xor<X>((uint32_t)(k >> 32)) << 32 | lane_xor<X>((uint32_t)k);
-}
-
-template <int X>
-__device__ inline void join_lanes(Sums& s) {
-  s.S += lane_xor_f<X>(s.S);
-  s.U += lane_xor_f<X>(s.U);
-  s.ahead += (int)lane_xor<X>((uint32_t)s.ahead);
-}
 __device__ inline Sums wave_join(Sums s) {
-  float m = s.m;
-  m = fmaxf(m, lane_xor_f<1>(m));
-  m = fmaxf(m, lane_xor_f<2>(m));
-  m = fmaxf(m, lane_xor_f<7>(m));
-  m = fmaxf(m, lane_xor_f<15>(m));
-  m = fmaxf(m, lane_xor_f<16>(m));
-  m = fmaxf(m, lane_xor_f<32>(m));
-  const float d = fmaxf(s.m - m, kFar), e = exp_of(d);
-  s.U = (s.U + s.S * d) * e;
-  s.S *= e;
+  const float m = wave_max(s.m), d = fmaxf(s.m - m, kFar), e = exp_of(d);
+  s.U = wave_sum((s.U + s.S * d) * e);
+  s.S = wave_sum(s.S * e);
   s.m = m;
-  join_lanes<1>(s);
-  join_lanes<2>(s);
-  join_lanes<7>(s);
-  join_lanes<15>(s);
-  join_lanes<16>(s);
-  join_lanes<32>(s);
+  int a = s.ahead;
+  a += (int)lane_xor<1>((uint32_t)a);
+  a += (int)lane_xor<2>((uint32_t)a);
+  a += (int)lane_xor<7>((uint32_t)a);
+  a += (int)lane_xor<15>((uint32_t)a);
+  a += (int)lane_xor<16>((uint32_t)a);
+  a += (int)lane_xor<32>((uint32_t)a);
+  s.ahead = a;
   return s;
 }
 
@@ -150,7 +108,8 @@ __device__ inline void halves16(u64& k) {
   exchange<2>(k);
   exchange<1>(k);
 }
-// 64 keys, descending over the lanes (a network whose merges begin mirrored).
+// 64 keys, descending over the lanes (a network whose merges begin mirrored; by way of LDS it
+// takes half as long again).
 __device__ inline u64 sort64(u64 k) {
   exchange<1>(k);
   exchange<3>(k);
