@@ -25,7 +25,13 @@
 // The values' columns are what the waves share out: each reads all four waves'
 // digits from LDS (12 KiB) and sums 256 tokens in integers before anything is
 // rounded.  A wave that kept all columns of its own tokens instead converted four
-// times as many sums, held 206 registers for 168, and ended in a join of the waves.
+// times as many sums, held 206 registers for 164, and ended in a join of the waves.
+//
+// What bounds it: many rows, the issue of VALU instructions beside the matrix ones (a
+// prompt's 512 rows of 8 heads a kv head at 1501 .. 2012: 42 us, VALU busy for 25 of them, MFMA
+// 10); a wave in its products goes before the other wave of its SIMD, so that one's products run
+// under the other's softmax (46 us without).  One row a sequence, two launches' latency and
+// then HBM (32 of 512 .. 4096 tokens, 54 MB: 21 us; one of 702: 7.9).
 //
 // The weights carry V's scale: with vs = f 2^e (1 <= f < 2), w_t = f 2^(s_t
 // log2(e) + e - M) against the running maximum M of these exponents, so the
@@ -47,6 +53,7 @@ constexpr int kWaves = 4;   // of a workgroup
 constexpr int kRound = kStep * kWaves;
 constexpr int kPages = 1024;  // blocks whose pages are held at a time: 64 rounds
 constexpr int kMaxParts = 1024;  // of a tile's tokens
+constexpr long kMostItems = 32768;  // workgroups with parts: what they leave stays below 600 MB
 constexpr int kJoinWave = 16;    // up to as many one wave joins a row
 constexpr float kNone = -INFINITY;
 // Weights below 2 become whole numbers below 2^23 - 0x8080: added to 2^23 +
@@ -353,6 +360,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
 #pragma unroll
     for (int r = 0; r < RT; r++) mx[r] = kNone;
     if (mine) {
+      __builtin_amdgcn_s_setprio(1);
       // Exponents: scores in powers of two, with V's.
       const float vs = sc.y;
       int ev = kMinExp;
@@ -397,12 +405,13 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     }
 #pragma unroll
     for (int r = 0; r < RT; r++) {
-      const float m = rows_max(mx[r]), s = rows_max(mx[r] - evf);
+      const float m = rows_larger(mx[r]), s = rows_larger(mx[r] - evf);
       if (g == 0) {
         smax[wave][r][n] = m;
         smaxs[wave][r][n] = s;
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     // This round's V, and behind it the next one's K.
     load_v(T0);
     const int Tn = T0 + kRound;
@@ -424,10 +433,10 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     float alpha[RT];
 #pragma unroll
     for (int r = 0; r < RT; r++) {
-      const float to = fmaxf(M[r], fmaxf(fmaxf(smax[0][r][n], smax[1][r][n]),
-                                         fmaxf(smax[2][r][n], smax[3][r][n])));
-      const float tos = fmaxf(N[r], fmaxf(fmaxf(smaxs[0][r][n], smaxs[1][r][n]),
-                                          fmaxf(smaxs[2][r][n], smaxs[3][r][n])));
+      const float to = larger(larger(larger(larger(M[r], smax[0][r][n]), smax[1][r][n]),
+                                     smax[2][r][n]), smax[3][r][n]);
+      const float tos = larger(larger(larger(larger(N[r], smaxs[0][r][n]), smaxs[1][r][n]),
+                                      smaxs[2][r][n]), smaxs[3][r][n]);
       const float ref = to == kNone ? 0.0f : to, refs = tos == kNone ? 0.0f : tos;
       alpha[r] = lift(M[r], ref);
       L[r] *= lift(N[r], refs);
@@ -463,6 +472,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
       }
     }
     __syncthreads();
+    __builtin_amdgcn_s_setprio(1);
     // Values: 256 tokens in integers (below 2^22, 2^30 with the next digit).
 #pragma unroll
     for (int r = 0; r < RT; r++) {
@@ -489,6 +499,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
           o[r][d][i] =
               __builtin_fmaf(o[r][d][i], alpha[r], joined(acc[d][2][i], acc[d][1][i], acc[d][0][i]));
     }
+    __builtin_amdgcn_s_setprio(0);
   }
 
   // The waves' denominators; then each wave has its columns' results.
@@ -673,7 +684,8 @@ AttnArgs attn_plan(const PoolView& p, const Ragged& r, int n_heads, int max_len,
   a.slots = r.T / a.qpt + a.extra * r.n;
   long range = max_len;
   if (window > 0 && window + (long)a.qpt + kStep < range) range = window + (long)a.qpt + kStep;
-  const long tiles = (r.T / a.qpt > r.n ? r.T / a.qpt : r.n) * (long)p.n_kv_heads * a.hgroups;
+  const long y = (long)p.n_kv_heads * a.hgroups;
+  const long tiles = (r.T / a.qpt > r.n ? r.T / a.qpt : r.n) * y;
   const float at_once = a.rt == 1 && p.hd <= 128 ? 768.0f : 512.0f, filled = r.n > 1 ? 0.6f : 1.0f;
   const long most = (range + kRound - 1) / kRound;
   float best = INFINITY;
@@ -681,7 +693,7 @@ AttnArgs attn_plan(const PoolView& p, const Ragged& r, int n_heads, int max_len,
   for (long rounds = 1;; rounds += 1 + rounds / 4) {
     if (rounds > most) rounds = most;
     const long parts = (most + rounds - 1) / rounds;
-    if (parts <= kMaxParts) {
+    if (parts == 1 || (parts <= kMaxParts && parts * a.slots * y <= kMostItems)) {
       const float wgs = (float)tiles * (float)parts;
       const float turns = parts > 1 ? wgs * filled / at_once : wgs / at_once;
       const float us = (turns > 1.0f ? turns : 1.0f) *

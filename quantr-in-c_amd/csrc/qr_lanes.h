@@ -55,12 +55,22 @@ __device__ inline void pair32(float v, float* x, float* y) {
   *x = __builtin_bit_cast(float, p);
   *y = __builtin_bit_cast(float, q);
 }
+// The larger of two numbers, NaN where one is: one instruction, where fmaxf of values that came
+// by way of memory or another lane takes three.
+__device__ inline float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 // Over the four lanes of equal lane % 16.
 __device__ inline float rows_max(float v) {
   float x, y;
   pair16(v, &x, &y);
   pair32(fmaxf(x, y), &x, &y);
   return fmaxf(x, y);
+}
+__device__ inline float rows_larger(float v) {
+  float x, y;
+  pair16(v, &x, &y);
+  pair32(larger(x, y), &x, &y);
+  return larger(x, y);
 }
 __device__ inline float rows_sum(float v) {
   float x, y;
