@@ -431,7 +431,8 @@ int qr_decoder_prefill(qr_decoder* dec, const int32_t* tokens, int n, int pos0, 
  * n_kv_heads up to 1024, max_pages * page up to 2^30.
  * Every call reads and writes them on the context's stream and waits for
  * nothing, so all of them can be captured into a graph (after one run that
- * grew the context's scratch).
+ * grew the context's scratch).  Calls of one context, and graphs captured from it,
+ * share that scratch: they must not run at once on two streams.
  *
  * A list argument (seqs, dst, ...) is a device array of n entries, n <=
  * QR_KV_MAX_LIST.  What a list asks for is checked on the device: `status`
@@ -464,7 +465,7 @@ int qr_kv_pool_reset(qr_ctx* ctx, const qr_kv_pool* pool);
 /* Sequence seqs[i] grows by add[i] tokens: it takes the pages that they need,
  * the free pages in ascending order in the order of the list.  Where its last
  * page is partly filled and shared, it first takes a copy of it (of all
- * layers): in the order of the list, each of them but the last that holds it. */
+ * layers): in the order of the list, each of them as long as another sequence holds it. */
 int qr_kv_pool_extend(qr_ctx* ctx, const qr_kv_pool* pool, const int32_t* seqs,
                       const int32_t* add, int n, int32_t* status);
 
@@ -489,7 +490,9 @@ int qr_kv_pool_compact(qr_ctx* ctx, const qr_kv_pool* pool, int32_t* map, int32_
 /* The rows of a ragged batch: T rows (at most QR_KV_MAX_ROWS), of which start[i] .. start[i + 1] - 1
  * (start: device int32 [n + 1], ascending) are sequence seqs[i]'s (seqs null:
  * sequence i's), n up to QR_KV_MAX_SEQS; they stand for its last positions, so a call that brings new
- * tokens extends first.  Rows that no sequence owns are left as they are.
+ * tokens extends first.  Rows that no sequence owns are left as they are.  A sequence that
+ * does not exist counts as empty.  `start` is not checked: entries outside 0 .. T are cut to it, and
+ * where they do not ascend results are undefined, but only rows below T are read or written.
  *
  * store quantizes K and V rows (fp32, head h's values at h * head_dim, row
  * stride kv_stride, a multiple of 4, 16-byte aligned) into layer `layer`.  A block's scale becomes
@@ -514,7 +517,8 @@ int qr_kv_pool_load(qr_ctx* ctx, const qr_kv_pool* pool, int layer, const int32_
  * aligned.  scale <= 0 means 1 / sqrtf(head_dim).  max_len bounds the
  * sequences' lengths for the split of the work (0: max_pages * page); longer
  * sequences are served all the same.  A row that sees no token (one before
- * position 0) gives zeros, a q row that is not finite NaN. */
+ * position 0) gives zeros, a q row that is not finite NaN.  A sequence may be listed more than
+ * once; out must not overlap q. */
 int qr_kv_pool_attention(qr_ctx* ctx, const qr_kv_pool* pool, int layer, const int32_t* seqs,
                          const int32_t* start, int n, int T, int n_heads, const float* q,
                          long q_stride, float* out, long out_stride, int max_len, int window,

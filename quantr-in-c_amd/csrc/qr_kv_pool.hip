@@ -907,6 +907,7 @@ int qr_kv_pool_attention(qr_ctx* c, const qr_kv_pool* p, int layer, const int32_
   const PoolView view = layer_view(p, layer);
   const int cap = p->max_pages * p->page;
   if (max_len == 0 || max_len > cap) max_len = cap;
+  if (window >= cap) window = 0;  // no sequence is longer
   void* w = nullptr;
   const size_t need = kv_attention_scratch(view, r, n_heads, max_len, window);
   if (need) {

@@ -372,6 +372,60 @@ def test_rows_before_the_first_sequence(dev):
             assert (x[:st[0]] == 7).all() and (x[st[-1]:] == 7).all()
 
 
+def test_windows_beyond_any_length(dev):
+    """The largest windows, with more rows than tokens, are no window."""
+    p = filled(41, [2, 300, 0], page=16, kv_heads=2, hd=64)
+    d = R.DevPool(dev, p)
+    none = check(d, p, [0, 1, 2], [5, 3, 2], 8, 3)
+    assert (none[:3] == 0).all() and (none[3:8] != 0).any() and (none[8:] == 0).all()
+    for window in (2 ** 31 - 1, 2 ** 30, 320, 319):
+        got = check(d, p, [0, 1, 2], [5, 3, 2], 8, 3, window=window)
+        np.testing.assert_array_equal(got.view(np.uint32), none.view(np.uint32))
+
+
+def test_a_sequence_listed_twice_is_read_twice(dev):
+    p = filled(42, [70, 45], page=32, kv_heads=2, hd=64)
+    d = R.DevPool(dev, p)
+    check(d, p, [0, 1, 0, 0], [3, 2, 1, 40], 4, 4)
+    k, v = d.load(0, [1, 1], starts([4, 2]), 6)
+    for got in (k, v):
+        np.testing.assert_array_equal(got[2:4], got[4:6])
+
+
+def test_many_sequences_under_a_loose_bound(dev):
+    """More tiles than parts are worth to, of a table for far longer sequences."""
+    rng = np.random.default_rng(43)
+    p = filled(43, [int(x) for x in rng.integers(0, 60, 300)], page=16, kv_heads=4, hd=32)
+    p.table = np.concatenate([p.table, np.full((300, 4096 - p.max_pages), -1, np.int32)], 1)
+    p.max_pages = 4096
+    check(R.DevPool(dev, p), p, list(range(300)), [1] * 300, 4, 6)
+
+
+def test_starts_that_are_not_ascending(dev):
+    """Whatever `start` holds, no row that is not there is read or written."""
+    p = filled(44, [90, 20, 40, 33], page=32, kv_heads=2, hd=64)
+    d = R.DevPool(dev, p)
+    rng = np.random.default_rng(7)
+    T, pad = 30, 4
+    x = rng.normal(0, 1, (T + pad, 4 * 64)).astype(np.float32)
+    for st in ([0, 20, 10, 2 ** 31 - 1, 5], [-2 ** 31, 30, -7, 12, 99], [31, 30, 29, 28, 27], [9] * 5,
+               [0, 30, 0, 30, 0]):
+        seqs, start = d.list([0, 1, 2, 3]), d.list(st)
+        q, kv = dev.upload(x), dev.upload(x[:, :128].copy())
+        out = dev.upload(np.full((T + pad, 256), 7, np.float32))
+        back = [dev.upload(np.full((T + pad, 128), 7, np.float32)) for _ in range(2)]
+        for max_len in (0, 16):
+            dev.kv_pool_attention(d.h, 0, seqs.ptr, start.ptr, 4, T, 4, q.ptr, out.ptr,
+                                  max_len=max_len)
+        dev.kv_pool_store(d.h, 0, seqs.ptr, start.ptr, 4, T, kv.ptr, kv.ptr)
+        dev.kv_pool_load(d.h, 0, seqs.ptr, start.ptr, 4, T, back[0].ptr, back[1].ptr)
+        got = dev.download(out, (T + pad, 256), np.float32)
+        assert np.isfinite(got).all() and (got[T:] == 7).all()
+        for b in back:
+            got = dev.download(b, (T + pad, 128), np.float32)
+            assert np.isfinite(got).all() and (got[T:] == 7).all()
+
+
 def test_attention_of_peaked_and_flat_scores(dev):
     p = filled(32, [500, 333], page=32, kv_heads=2, hd=128)
     d = R.DevPool(dev, p)
