@@ -518,11 +518,14 @@ __global__ __launch_bounds__(256) void k_pool_store(PoolView p, Ragged r, const 
   if (side == 0) {
     constexpr int Q = HD / 4, N = (kKvBlock * Q + 63) / 64;
     float4 f[N];
+    int old[N];
 #pragma unroll
     for (int j = 0; j < N; j++) {
       const int e = lane + 64 * j, t = e / Q;
       f[j] = make_float4(0, 0, 0, 0);
+      old[j] = 0;
       if (e < kKvBlock * Q && fresh(t)) f[j] = *reinterpret_cast<const float4*>(row(t) + e % Q * 4);
+      if (e < kKvBlock * Q && t < b.first) old[j] = reinterpret_cast<const int*>(out)[e];
     }
 #pragma unroll
     for (int j = 0; j < N; j++) {
@@ -543,7 +546,7 @@ __global__ __launch_bounds__(256) void k_pool_store(PoolView p, Ragged r, const 
                   d = quantized(f[j].z, s, inv, tiny), g = quantized(f[j].w, s, inv, tiny);
         *o = (a & 255) | (c & 255) << 8 | (d & 255) << 16 | g << 24;
       } else if (grew && t < b.first) {
-        const int u = *o;
+        const int u = old[j];
         const int a = requantized((int8_t)u, was, s), c = requantized((int8_t)(u >> 8), was, s),
                   d = requantized((int8_t)(u >> 16), was, s), g = requantized(u >> 24, was, s);
         *o = (a & 255) | (c & 255) << 8 | (d & 255) << 16 | g << 24;
@@ -552,6 +555,14 @@ __global__ __launch_bounds__(256) void k_pool_store(PoolView p, Ragged r, const 
   } else {
     constexpr int N = (HD + 63) / 64;
     float f[N][kKvBlock];
+    int4 old[N];
+    const bool all = b.first <= 0 && b.s.m + b.first >= kKvBlock;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const int c = lane + 64 * j;
+      old[j] = make_int4(0, 0, 0, 0);
+      if (!all && c < HD) old[j] = *reinterpret_cast<const int4*>(out + c * kKvBlock);
+    }
 #pragma unroll
     for (int j = 0; j < N; j++)
 #pragma unroll
@@ -570,14 +581,7 @@ __global__ __launch_bounds__(256) void k_pool_store(PoolView p, Ragged r, const 
       const int c = lane + 64 * j;
       if (c >= HD) continue;
       int4* o = reinterpret_cast<int4*>(out + c * kKvBlock);
-      int u[4] = {0, 0, 0, 0};
-      if (!(b.first <= 0 && b.s.m + b.first >= kKvBlock)) {
-        const int4 old = *o;
-        u[0] = old.x;
-        u[1] = old.y;
-        u[2] = old.z;
-        u[3] = old.w;
-      }
+      int u[4] = {old[j].x, old[j].y, old[j].z, old[j].w};
 #pragma unroll
       for (int t = 0; t < kKvBlock; t++) {
         int q = (int8_t)(u[t >> 2] >> 8 * (t & 3));
@@ -615,22 +619,35 @@ __global__ __launch_bounds__(256) void k_pool_load(PoolView p, Ragged r, float* 
   auto row = [&](int t) { return x + (size_t)(b.s.row0 + t - b.first) * stride; };
   if (side == 0) {
     constexpr int Q = HD / 4, N = (kKvBlock * Q + 63) / 64;
+    int block[N];
 #pragma unroll
     for (int j = 0; j < N; j++) {
-      const int e = lane + 64 * j, t = e / Q;
+      const int e = lane + 64 * j;
+      block[j] = e < kKvBlock * Q ? reinterpret_cast<const int*>(in)[e] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const int e = lane + 64 * j, t = e / Q, u = block[j];
       if (e >= kKvBlock * Q || !fresh(t)) continue;
-      const int u = reinterpret_cast<const int*>(in)[e];
       *reinterpret_cast<float4*>(row(t) + e % Q * 4) =
           make_float4((float)(int8_t)u * s, (float)(int8_t)(u >> 8) * s,
                       (float)(int8_t)(u >> 16) * s, (float)(u >> 24) * s);
     }
   } else {
-    for (int c = lane; c < HD; c += 64) {
-      const int4 o = *reinterpret_cast<const int4*>(in + c * kKvBlock);
-      const int u[4] = {o.x, o.y, o.z, o.w};
+    constexpr int N = (HD + 63) / 64;
+    int4 block[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const int c = lane + 64 * j;
+      block[j] = make_int4(0, 0, 0, 0);
+      if (c < HD) block[j] = *reinterpret_cast<const int4*>(in + c * kKvBlock);
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const int c = lane + 64 * j, u[4] = {block[j].x, block[j].y, block[j].z, block[j].w};
 #pragma unroll
       for (int t = 0; t < kKvBlock; t++)
-        if (fresh(t)) row(t)[c] = (float)(int8_t)(u[t >> 2] >> 8 * (t & 3)) * s;
+        if (c < HD && fresh(t)) row(t)[c] = (float)(int8_t)(u[t >> 2] >> 8 * (t & 3)) * s;
     }
   }
 }
