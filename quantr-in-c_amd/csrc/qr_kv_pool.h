@@ -48,7 +48,7 @@ struct SeqRows {
 };
 __device__ inline int seq_len(const PoolView& p, const SeqRows& s) {
   const long cap = (long)p.max_pages << p.page_shift;
-  const int n = p.len[s.seq];
+  const int n = __builtin_amdgcn_readfirstlane(p.len[s.seq]);
   return !s.there || n < 0 ? 0 : n > cap ? (int)cap : n;
 }
 

@@ -456,32 +456,46 @@ __device__ inline BlockRows block_rows(const PoolView& p, const Ragged& r, int s
   return b;
 }
 
-// x / s rounded to the nearest even integer, for a normal s and |x| <= 127 s
-// but for rounding.  The product with 1 / s is within one integer of it, and
-// what it leaves of x is a multiple of the smaller of both ulps below 2^24 of
-// them, so the fused multiply-add forms it exactly and decides.
-__device__ inline float quotient(float x, float s, float inv) {
-  const float q = rintf(x * inv);
-  const float rem = __builtin_fmaf(-q, s, x), two = 2.0f * fabsf(rem);
-  const bool odd = ((int)q & 1) != 0;
-  return two > s || (two == s && odd) ? q + copysignf(1.0f, rem) : q;
+// A block's scale, and what its values and its older scale are multiplied by (a power of two)
+// so that nothing below under- or overflows.
+struct Step {
+  float s, inv, mul, was;
+};
+__device__ inline Step step_of(float s, float was) {
+  Step k;
+  k.mul = s < 0x1p-100f ? 0x1p100f : s > 0x1p100f ? 0x1p-100f : 1.0f;
+  k.s = s * k.mul;
+  k.was = was * k.mul;
+  k.inv = 1.0f / k.s;
+  return k;
 }
 
-__device__ inline int quantized(float x, float s, float inv, bool tiny) {
-  float q;
-  if (tiny)
-    q = (float)rint((double)x / (double)s);
-  else
-    q = quotient(x, s, inv);
+// x / s rounded to the nearest even integer, for |x| <= 127 s but for rounding.  The
+// product with 1 / s is within one integer of it, and what it leaves of x is a multiple of the
+// smaller of both ulps below 2^24 of them, so the fused multiply-add forms it
+// exactly and decides.
+__device__ inline int quantized(float x, const Step& k) {
+  const float y = x * k.mul;
+  float q = rintf(y * k.inv);
+  const float rem = __builtin_fmaf(-q, k.s, y), two = 2.0f * fabsf(rem);
+  const bool odd = ((int)q & 1) != 0;
+  q += (two > k.s) | ((two == k.s) & odd) ? copysignf(1.0f, rem) : 0.0f;
   q = fminf(fmaxf(q, -127.0f), 127.0f);
   if (!(fabsf(x) <= 3.402823466e+38f)) q = x != x ? 0.0f : copysignf(127.0f, x);
-  return s > 0.0f ? (int)q : 0;
+  return k.s > 0.0f ? (int)q : 0;
 }
 
-// An older value under a grown scale.  A quotient of a 31-bit and a 24-bit
-// integer is 2^-33 or more from a half unless it is one, so 64 bits decide.
-__device__ inline int requantized(int q, float was, float now) {
-  return (int)rint((double)q * (double)was / (double)now);
+// An older value under a grown scale, rounded the same way.  Its product with the old scale
+// is p + e exactly; where the rest r of p is near half a step, 2 r - s is exact, and the sign of
+// its sum with 2 e decides.
+__device__ inline int requantized(int q, const Step& k) {
+  const float a = fabsf((float)q), p = a * k.was, e = __builtin_fmaf(a, k.was, -p);
+  float m = rintf(p * k.inv);
+  const float r = __builtin_fmaf(-m, k.s, p);
+  const float over = __builtin_fmaf(2.0f, fabsf(r), -k.s) + copysignf(2.0f, r) * e;
+  const bool odd = ((int)m & 1) != 0;
+  m += (over > 0.0f) | ((over == 0.0f) & odd) ? copysignf(1.0f, r) : 0.0f;
+  return q < 0 ? -(int)m : (int)m;
 }
 
 // A wave per (block, kv head, K or V): its new rows in registers, the largest
@@ -493,7 +507,7 @@ template <int HD>
 __global__ __launch_bounds__(256) void k_pool_store(PoolView p, Ragged r, const float* k,
                                                     const float* v, long stride, int slots) {
   const int lane = threadIdx.x & 63;
-  const int w = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int w = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int side = w & 1, slot = w >> 1, kvh = blockIdx.y;
   if (slot >= slots) return;
   const BlockRows b = block_rows(p, r, slot, kvh);
@@ -534,22 +548,25 @@ __global__ __launch_bounds__(256) void k_pool_store(PoolView p, Ragged r, const 
       take(f[j].z);
       take(f[j].w);
     }
-    const float s = scale_of(), inv = 1.0f / s;
-    const bool tiny = s < 1e-36f, grew = held && s > was;
+    const float s = scale_of();
+    const Step st = step_of(s, was);
+    const bool grew = held && s > was;
 #pragma unroll
     for (int j = 0; j < N; j++) {
-      const int e = lane + 64 * j, t = e / Q;
-      if (e >= kKvBlock * Q) continue;
-      int* o = reinterpret_cast<int*>(out) + e;
-      if (fresh(t)) {
-        const int a = quantized(f[j].x, s, inv, tiny), c = quantized(f[j].y, s, inv, tiny),
-                  d = quantized(f[j].z, s, inv, tiny), g = quantized(f[j].w, s, inv, tiny);
-        *o = (a & 255) | (c & 255) << 8 | (d & 255) << 16 | g << 24;
-      } else if (grew && t < b.first) {
-        const int u = old[j];
-        const int a = requantized((int8_t)u, was, s), c = requantized((int8_t)(u >> 8), was, s),
-                  d = requantized((int8_t)(u >> 16), was, s), g = requantized(u >> 24, was, s);
-        *o = (a & 255) | (c & 255) << 8 | (d & 255) << 16 | g << 24;
+      const int e = lane + 64 * j;
+      const int a = quantized(f[j].x, st), c = quantized(f[j].y, st), d = quantized(f[j].z, st),
+                g = quantized(f[j].w, st);
+      if (e < kKvBlock * Q && fresh(e / Q))
+        reinterpret_cast<int*>(out)[e] = (a & 255) | (c & 255) << 8 | (d & 255) << 16 | g << 24;
+    }
+    if (grew) {
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        const int e = lane + 64 * j, u = old[j];
+        const int a = requantized((int8_t)u, st), c = requantized((int8_t)(u >> 8), st),
+                  d = requantized((int8_t)(u >> 16), st), g = requantized(u >> 24, st);
+        if (e < kKvBlock * Q && e / Q < b.first)
+          reinterpret_cast<int*>(out)[e] = (a & 255) | (c & 255) << 8 | (d & 255) << 16 | g << 24;
       }
     }
   } else {
@@ -574,24 +591,25 @@ __global__ __launch_bounds__(256) void k_pool_store(PoolView p, Ragged r, const 
     for (int j = 0; j < N; j++)
 #pragma unroll
       for (int t = 0; t < kKvBlock; t++) take(f[j][t]);
-    const float s = scale_of(), inv = 1.0f / s;
-    const bool tiny = s < 1e-36f, grew = held && s > was;
+    const float s = scale_of();
+    const Step st = step_of(s, was);
+    const bool grew = held && s > was;
 #pragma unroll
     for (int j = 0; j < N; j++) {
       const int c = lane + 64 * j;
-      if (c >= HD) continue;
-      int4* o = reinterpret_cast<int4*>(out + c * kKvBlock);
       int u[4] = {old[j].x, old[j].y, old[j].z, old[j].w};
-#pragma unroll
-      for (int t = 0; t < kKvBlock; t++) {
-        int q = (int8_t)(u[t >> 2] >> 8 * (t & 3));
-        if (fresh(t))
-          q = quantized(f[j][t], s, inv, tiny);
-        else if (grew && t < b.first)
-          q = requantized(q, was, s);
+      auto put = [&](int t, int q) {
         u[t >> 2] = (u[t >> 2] & ~(255 << 8 * (t & 3))) | (q & 255) << 8 * (t & 3);
+      };
+      if (grew) {
+#pragma unroll
+        for (int t = 0; t < kKvBlock; t++)
+          if (t < b.first) put(t, requantized((int8_t)(u[t >> 2] >> 8 * (t & 3)), st));
       }
-      *o = make_int4(u[0], u[1], u[2], u[3]);
+#pragma unroll
+      for (int t = 0; t < kKvBlock; t++)
+        if (fresh(t)) put(t, quantized(f[j][t], st));
+      if (c < HD) *reinterpret_cast<int4*>(out + c * kKvBlock) = make_int4(u[0], u[1], u[2], u[3]);
     }
   }
 }
@@ -602,7 +620,7 @@ template <int HD>
 __global__ __launch_bounds__(256) void k_pool_load(PoolView p, Ragged r, float* k, float* v,
                                                    long stride, int slots) {
   const int lane = threadIdx.x & 63;
-  const int w = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int w = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int side = w & 1, slot = w >> 1, kvh = blockIdx.y;
   if (slot >= slots) return;
   float* x = (side ? v : k) + (size_t)kvh * HD;
