@@ -428,7 +428,8 @@ int qr_decoder_prefill(qr_decoder* dec, const int32_t* tokens, int n, int pos0, 
  *   len    int32 [n_seqs]: the tokens of each sequence;
  *   refs   int32 [n_pages]: the table entries that name a page (0: free).
  * page is a power of two from 16 to 65536, head_dim a multiple of 32 up to 256,
- * n_kv_heads up to 1024, max_pages * page up to 2^30.
+ * n_kv_heads up to 1024, max_pages * page up to 2^30, n_pages * n_kv_heads *
+ * (page / 16) up to 2^31.
  * Every call reads and writes them on the context's stream and waits for
  * nothing, so all of them can be captured into a graph (after one run that
  * grew the context's scratch).  Calls of one context, and graphs captured from it,

@@ -83,7 +83,7 @@ struct AttnArgs {
   const float* q;
   float* out;
   long q_stride, out_stride;
-  int n_heads, group;   // query heads, query heads per kv head
+  int group;            // query heads per kv head
   int hgroups, hpt;     // groups of at most 16 of a kv head's query heads, heads of each
   int rt, qpt, extra;   // 16-row sets of a tile, queries of it, slots beyond T / qpt for each sequence
   int slots, splits;    // tiles of a head group, parts that a tile's tokens are cut into
@@ -204,7 +204,13 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
   }
   // What hangs on the sequence alone is fetched together: the first round's pages where no window
   // moves it (one of its 16 blocks in each lane group's lanes; -1: none), q, the length.
-  auto pages = [&](int T0) { return page_at(a.p, t.seq, (T0 + 16 * n) >> a.p.page_shift); };
+  // Pages stand for the first of this kv head's blocks in them: below 2^31 in a layer.
+  const int pshift = a.p.page_shift - 4, pmask = (1 << pshift) - 1;
+  auto page_of = [&](int T0) {
+    const int g = page_at(a.p, t.seq, T0 >> a.p.page_shift);
+    return g < 0 ? -1 : (g * a.p.n_kv_heads + kvh) << pshift;
+  };
+  auto pages = [&](int T0) { return page_of(T0 + 16 * n); };
   int pg = -1;
   if (a.window == 0) pg = pages(z * a.chunk);
   // q: kPer lanes share a row, four columns each; a wave takes every fourth set of rows.
@@ -234,11 +240,10 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
   // loop would wait for the V before it.
   auto fill_pages = [&](int T0) {
     for (int i = threadIdx.x; i < kPages && T0 + 16 * i < te; i += 256)
-      spg[i] = page_at(a.p, t.seq, (T0 + 16 * i) >> a.p.page_shift);
+      spg[i] = page_of(T0 + 16 * i);
   };
   const bool more = tb + kRound < te;
   if (more) fill_pages(tb);
-  const int pmask = (1 << (a.p.page_shift - 4)) - 1;
   const int8_t* const data = a.p.data;
 
   // this lane's rows
@@ -263,10 +268,12 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
   bool here;
   const int kb = 4 * wave + (n >> 2);  // the round's block of the lane's K rows
   int kp = -1, wp = -1, vp[kWaves];  // pages of its K, its scales, and V's four blocks
+  // What is not there: the first page's.
+  auto block = [&](int page, int b) { return (uint32_t)((page < 0 ? 0 : page) + (b & pmask)); };
   auto load_k = [&](int T0) {
     const int b0 = T0 >> 4;
-    const size_t bk = block_at(a.p, kp < 0 ? 0 : kp, kvh, (b0 + kb) & pmask);
-    const int8_t* s = data + bk * (2 * kKvBlock * HD) + (n & 3) * HD + (16 * g < HD ? 16 * g : 0);
+    const int8_t* s = data + (size_t)block(kp, b0 + kb) * (2 * kKvBlock * HD) + (n & 3) * HD +
+                      (16 * g < HD ? 16 * g : 0);
 #pragma unroll
     for (int tt = 0; tt < 4; tt++)
 #pragma unroll
@@ -276,14 +283,13 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     here = wp >= 0;
     sc = make_float2(0.0f, 0.0f);
     if (here)
-      sc = *reinterpret_cast<const float2*>(
-          a.p.scale + 2 * block_at(a.p, wp, kvh, (b0 + 4 * wave + g) & pmask));
+      sc = reinterpret_cast<const float2*>(a.p.scale)[block(wp, b0 + 4 * wave + g)];
   };
   auto load_v = [&](int T0) {
 #pragma unroll
     for (int s = 0; s < kWaves; s++) {
-      const size_t bv = block_at(a.p, vp[s] < 0 ? 0 : vp[s], kvh, ((T0 >> 4) + 4 * s + g) & pmask);
-      const int8_t* v = data + bv * (2 * kKvBlock * HD) + kKvBlock * HD + n * kKvBlock;
+      const int8_t* v = data + (size_t)block(vp[s], (T0 >> 4) + 4 * s + g) * (2 * kKvBlock * HD) +
+                        kKvBlock * HD + n * kKvBlock;
 #pragma unroll
       for (int d = 0; d < NV; d++)
         if (HD % 64 == 0 || wave + 4 * d < HD / 16)
@@ -669,7 +675,6 @@ AttnArgs attn_plan(const PoolView& p, const Ragged& r, int n_heads, int max_len,
   AttnArgs a = {};
   a.p = p;
   a.r = r;
-  a.n_heads = n_heads;
   a.group = n_heads / p.n_kv_heads;
   a.hgroups = (a.group + 15) / 16;
   a.hpt = (a.group + a.hgroups - 1) / a.hgroups;

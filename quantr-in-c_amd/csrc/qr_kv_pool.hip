@@ -686,6 +686,8 @@ int pool_check(const qr_ctx* c, const qr_kv_pool* p, const char* who) {
   if ((long)p->max_pages * p->page > 1l << 30)
     return set_error(QR_ERR_INVALID, "%s: %d pages of %d tokens exceed 2^30", who, p->max_pages,
                      p->page);
+  if ((long)p->n_pages * p->n_kv_heads * (p->page / kKvBlock) > 1l << 31)
+    return set_error(QR_ERR_INVALID, "%s: more than 2^31 blocks a layer", who);
   if (!p->data || !p->scale || !p->table || !p->len || !p->refs)
     return set_error(QR_ERR_INVALID, "%s: null pointer in the pool", who);
   if (((uintptr_t)p->data & 15) || ((uintptr_t)p->scale & 7) || ((uintptr_t)p->table & 3) ||

@@ -51,7 +51,8 @@ def test_pools_that_cannot_be(name):
             (dict(n_layers=0), "layers"), (dict(n_pages=-1), "pages"), (dict(n_kv_heads=0), "heads"),
             (dict(n_kv_heads=1025), "heads"), (dict(n_seqs=0), "table"),
             (dict(n_seqs=65537), "table"), (dict(max_pages=0), "table"),
-            (dict(max_pages=(1 << 25) + 1), "2^30"), (dict(data=None), "null"), (dict(scale=None), "null"),
+            (dict(max_pages=(1 << 25) + 1), "2^30"), (dict(n_pages=(1 << 29) + 1, page=32), "2^31"),
+            (dict(data=None), "null"), (dict(scale=None), "null"),
             (dict(table=None), "null"), (dict(len=None), "null"), (dict(refs=None), "null"),
             (dict(data=BASE + 8), "alignment"), (dict(scale=BASE + 4), "alignment"),
             (dict(table=BASE + 2), "alignment")):
