@@ -34,10 +34,12 @@
 // then HBM (32 of 512 .. 4096 tokens, 54 MB: 21 us; one of 702: 7.9).
 //
 // The weights carry V's scale: with vs = f 2^e (1 <= f < 2), w_t = f 2^(s_t
-// log2(e) + e - M) against the running maximum M of these exponents, so the
-// digits are taken from the numbers that are summed.  The denominator runs
-// against the maximum N of the scores alone, its terms the same powers times 2^(M - e
-// - N): values of V however unlike move no token out of it.
+// log2(e) + e - M) against a reference M that brings the round's largest weight just
+// below 1 (more than 2^kFall below the row's largest it does not follow), so the
+// digits are taken from the numbers that are summed and hold them to 2^-24 of the largest
+// of 256.  The denominator runs against the maximum N of the scores alone, its
+// terms the same powers times 2^(M - e - N): values of V however unlike move no token out
+// of it.
 #include <math.h>
 
 #include "qr_kv_pool.h"
@@ -56,10 +58,10 @@ constexpr int kMaxParts = 1024;  // of a tile's tokens
 constexpr long kMostItems = 32768;  // workgroups with parts: what they leave stays below 600 MB
 constexpr int kJoinWave = 16;    // up to as many one wave joins a row
 constexpr float kNone = -INFINITY;
-// Weights below 2 become whole numbers below 2^23 - 0x8080: added to 2^23 +
+// Weights up to 1 become whole numbers below 2^23 - 0x8080: added to 2^23 +
 // 0x8080 they are the low mantissa bits of a float, and its three low bytes the
 // digits but for the 0x80 that the two lower bytes carry.
-constexpr float kWMul = 4177800.0f;
+constexpr float kWMul = 8355600.0f;
 constexpr float kWAdd = 8388608.0f + 32896.0f;
 constexpr float kQMax = 8355711.0f;  // 127 * (65536 + 256 + 1)
 // Exponent of V scales that are 0 or smaller than it: such a block's weights
@@ -68,6 +70,7 @@ constexpr int kMinExp = -60;
 // A block whose exponents lie further below M takes its powers 2^-kDeep below them, so that
 // they are there for the denominator.
 constexpr float kDeep = 60.0f;
+constexpr float kFall = 24.0f;
 
 // Where the rows of tile `slot` come from.
 struct Tile {
@@ -167,6 +170,15 @@ __device__ inline float joined(int s2, int s1, int s0) {
 
 __device__ inline int4 load16(const int8_t* p) { return *reinterpret_cast<const int4*>(p); }
 __device__ inline v4i as_v4(int4 x) { return v4i{x.x, x.y, x.z, x.w}; }
+
+// The reference for weights up to 2^x: the next multiple of 1 / 16, so that the references'
+// and V's exponents differ by what fp32 holds exactly and no rounding of theirs moves a
+// whole block or row.  Above x by what rounding may have taken from x; from 2^20 on no
+// multiple.
+__device__ inline float reference(float x) {
+  const float y = __builtin_fmaf(fabsf(x), 0x1p-22f, x), r = ceilf(y * 16.0f) * 0.0625f;
+  return x == kNone ? kNone : __builtin_amdgcn_fmed3f(r, y, fmaxf(y, 1048576.0f));
+}
 
 // The factor that takes a sum against maximum m to one against `to`.
 __device__ inline float lift(float m, float to) {
@@ -348,9 +360,10 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
   for (int r = 0; r < RT; r++) qs[r] = sqs[16 * r + n];
 
   float o[RT][NV][4], M[RT], N[RT], L[RT];
+  float top[RT];  // the largest weight's power so far
 #pragma unroll
   for (int r = 0; r < RT; r++) {
-    M[r] = N[r] = kNone;
+    M[r] = N[r] = top[r] = kNone;
     L[r] = 0.0f;
 #pragma unroll
     for (int d = 0; d < NV; d++)
@@ -362,7 +375,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     const int Tw = T0 + wave * kStep;  // of the wave
     const bool mine = Tw < te;
     float e[RT][16], mx[RT];  // exponents, and their largest of the lane's block
-    float evf = 0.0f, fw = 0.0f;
+    float evf = 0.0f, fw = 0.0f, lf = 0.0f;
 #pragma unroll
     for (int r = 0; r < RT; r++) mx[r] = kNone;
     if (mine) {
@@ -371,7 +384,9 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
       const float vs = sc.y;
       int ev = kMinExp;
       if (vs > 0x1p-60f) ev = (int)((__builtin_bit_cast(uint32_t, vs) >> 23) & 255) - 127;
-      fw = vs * __builtin_bit_cast(float, (uint32_t)(127 - ev) << 23) * kWMul;
+      const float f = vs * __builtin_bit_cast(float, (uint32_t)(127 - ev) << 23);
+      fw = f * kWMul;
+      lf = fmaxf(__builtin_amdgcn_logf(f), 0.0f);
       evf = (float)ev;
       // Every token of the step seen by every row of the tile?
       const bool full = __all(here) && Tw + kStep <= t.pos0 + 1 &&
@@ -411,7 +426,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     }
 #pragma unroll
     for (int r = 0; r < RT; r++) {
-      const float m = rows_larger(mx[r]), s = rows_larger(mx[r] - evf);
+      const float m = rows_larger(mx[r] + lf), s = rows_larger(mx[r] - evf);
       if (g == 0) {
         smax[wave][r][n] = m;
         smaxs[wave][r][n] = s;
@@ -439,10 +454,12 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     float alpha[RT];
 #pragma unroll
     for (int r = 0; r < RT; r++) {
-      const float to = larger(larger(larger(larger(M[r], smax[0][r][n]), smax[1][r][n]),
-                                     smax[2][r][n]), smax[3][r][n]);
-      const float tos = larger(larger(larger(larger(N[r], smaxs[0][r][n]), smaxs[1][r][n]),
-                                      smaxs[2][r][n]), smaxs[3][r][n]);
+      const float round = larger(larger(larger(smax[0][r][n], smax[1][r][n]), smax[2][r][n]),
+                                 smax[3][r][n]);
+      top[r] = larger(top[r], round);
+      const float to = reference(larger(round, top[r] - kFall));
+      const float tos = reference(larger(larger(larger(larger(N[r], smaxs[0][r][n]),
+                                                       smaxs[1][r][n]), smaxs[2][r][n]), smaxs[3][r][n]));
       const float ref = to == kNone ? 0.0f : to, refs = tos == kNone ? 0.0f : tos;
       alpha[r] = lift(M[r], ref);
       L[r] *= lift(N[r], refs);

@@ -434,6 +434,23 @@ def test_attention_of_peaked_and_flat_scores(dev):
         check(d, p, [0, 1], [2, 1], 8, 5, std=std, scale=scale)
 
 
+def test_attention_of_sinks(dev):
+    """A token whose score leads all others by 2^5 to 2^90, first, last or amid rounds
+    of 256 others, whose values are far smaller or larger than its own."""
+    hd = 64
+    for at, lead, own in ((0, 4.0, 1.0), (0, 20.0, 1.0), (0, 60.0, 1.0), (1200, 20.0, 1.0),
+                          (700, 12.0, 1e-6), (0, 14.0, 1e-9), (300, 40.0, 1e-30), (0, 20.0, 1e6)):
+        p = filled(45, [1201], page=32, kv_heads=1, hd=hd)
+        q = np.random.default_rng(9).normal(0, 1, (1, 2 * hd)).astype(np.float32)
+        g, b = p.table[0, at // 32], at // 16 % 2
+        k = np.rint(127 * q[0, :hd] / np.abs(q[0, :hd]).max())
+        p.data[0, g, 0, b, 0].reshape(16, hd)[at % 16] = k
+        # the scale that gives it a score of lead + 4 (times ln 2 or so) for the first head
+        p.scale[0, g, 0, b, 0] = (lead + 4) * np.sqrt(hd) / float(k @ q[0, :hd])
+        p.scale[0, g, 0, b, 1] = 0.02 * own
+        check(R.DevPool(dev, p), p, [0], [1], 2, 9)
+
+
 def test_attention_of_unlike_blocks(dev):
     """Blocks of zeros, of the smallest and of large values beside ordinary ones."""
     p = filled(33, [200], page=32, kv_heads=1, hd=64)
