@@ -28,10 +28,10 @@
 // times as many sums, held 206 registers for 164, and ended in a join of the waves.
 //
 // What bounds it: many rows, the issue of VALU instructions beside the matrix ones (a
-// prompt's 512 rows of 8 heads a kv head at 1501 .. 2012: 42 us, VALU busy for 25 of them, MFMA
-// 10); a wave in its products goes before the other wave of its SIMD, so that one's products run
-// under the other's softmax (46 us without).  One row a sequence, two launches' latency and
-// then HBM (32 of 512 .. 4096 tokens, 54 MB: 21 us; one of 702: 7.9).
+// prompt's 512 rows of 8 heads a kv head at 1501 .. 2012: 42 us, VALU busy for 23 of them, MFMA
+// 9); a wave in its products goes before the other wave of its SIMD, so that one's products run
+// under the other's softmax (46 us without it).  One row a sequence, two launches' latency and
+// then HBM (32 of 512 .. 4096 tokens, 54 MB: 21 us; one of 702: 8.0).
 //
 // The weights carry V's scale: with vs = f 2^e (1 <= f < 2), w_t = f 2^(s_t
 // log2(e) + e - M) against a reference M that brings the round's largest weight just
