@@ -33,7 +33,7 @@
 // under the other's softmax (46 us without it).  One row a sequence, two launches' latency and
 // then HBM (32 of 512 .. 4096 tokens, 54 MB: 21 us; one of 702: 8.0).
 //
-// The weights carry V's scale: with vs = f 2^e (1 <= f < 2), w_t = f 2^(s_t
+// The weights carry V's scale: with vs = f 2^e (1/2 <= f < 1), w_t = f 2^(s_t
 // log2(e) + e - M) against a reference M that brings the round's largest weight just
 // below 1 (more than 2^kFall below the row's largest it does not follow), so the
 // digits are taken from the numbers that are summed and hold them to 2^-24 of the largest
@@ -173,11 +173,11 @@ __device__ inline v4i as_v4(int4 x) { return v4i{x.x, x.y, x.z, x.w}; }
 
 // The reference for weights up to 2^x: the next multiple of 1 / 16, so that the references'
 // and V's exponents differ by what fp32 holds exactly and no rounding of theirs moves a
-// whole block or row.  Above x by what rounding may have taken from x; from 2^20 on no
-// multiple.
+// whole block or row, above x by what rounding may have taken from x.  From kLarge on x itself.
+constexpr float kLarge = 1048576.0f;
 __device__ inline float reference(float x) {
-  const float y = __builtin_fmaf(fabsf(x), 0x1p-22f, x), r = ceilf(y * 16.0f) * 0.0625f;
-  return x == kNone ? kNone : __builtin_amdgcn_fmed3f(r, y, fmaxf(y, 1048576.0f));
+  const float r = ceilf(__builtin_fmaf(fabsf(x), 0x1p-22f, x) * 16.0f) * 0.0625f;
+  return fabsf(x) < kLarge ? r : x;
 }
 
 // The factor that takes a sum against maximum m to one against `to`.
@@ -383,10 +383,13 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
       // Exponents: scores in powers of two, with V's.
       const float vs = sc.y;
       int ev = kMinExp;
-      if (vs > 0x1p-60f) ev = (int)((__builtin_bit_cast(uint32_t, vs) >> 23) & 255) - 127;
-      const float f = vs * __builtin_bit_cast(float, (uint32_t)(127 - ev) << 23);
+      float f = vs * 0x1p60f;
+      if (vs > 0x1p-60f) {
+        ev = __builtin_amdgcn_frexp_expf(vs);
+        f = __builtin_amdgcn_frexp_mantf(vs);
+      }
       fw = f * kWMul;
-      lf = fmaxf(__builtin_amdgcn_logf(f), 0.0f);
+      lf = fmaxf(__builtin_amdgcn_logf(f), -1.0f);
       evf = (float)ev;
       // Every token of the step seen by every row of the tile?
       const bool full = __all(here) && Tw + kStep <= t.pos0 + 1 &&
@@ -426,7 +429,11 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     }
 #pragma unroll
     for (int r = 0; r < RT; r++) {
-      const float m = rows_larger(mx[r] + lf), s = rows_larger(mx[r] - evf);
+      // Powers so large that f (V's exponent) is within their rounding: without it, which errs to
+      // the safe side (and for N, any number near the scores' largest will do).
+      const float x = fabsf(mx[r]);
+      const float m = rows_larger(x < kLarge ? mx[r] + lf : mx[r]);
+      const float s = rows_larger(x < 0x1p24f ? mx[r] - evf : mx[r]);
       if (g == 0) {
         smax[wave][r][n] = m;
         smaxs[wave][r][n] = s;
@@ -468,7 +475,8 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
       if (mine) {
         // 0 but for blocks far below M (and 300 for those that nothing is seen of)
         const float deep = fminf(fmaxf(ceilf(ref - mx[r]) - kDeep, 0.0f), 300.0f);
-        const float base = ref - deep, fwd = __builtin_ldexpf(fw, -(int)deep);
+        const float base = ref - deep, down = ref - base;
+        const float fwd = __builtin_ldexpf(fw, -(int)down);
         float sum = 0.0f;
         int4 p[3];
         int* d0 = &p[0].x;
@@ -485,7 +493,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
           }
           digits4(u[0], u[1], u[2], u[3], d0 + tt, d1 + tt, d2 + tt);
         }
-        L[r] = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(base - evf - refs), L[r]);
+        L[r] = __builtin_fmaf(sum, __builtin_amdgcn_exp2f((ref - refs) - down - evf), L[r]);
 #pragma unroll
         for (int k = 0; k < 3; k++) sp[wave][r][k][lane] = p[k];
       } else {

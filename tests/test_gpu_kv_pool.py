@@ -434,6 +434,36 @@ def test_attention_of_peaked_and_flat_scores(dev):
         check(d, p, [0, 1], [2, 1], 8, 5, std=std, scale=scale)
 
 
+@pytest.mark.parametrize("std", [3e4, 4e5, 3e6, 2e7, 1e8, 3e9, 1e12, 1e30])
+def test_attention_of_huge_scores(dev, std):
+    """Scores far apart for fp32's spacing at their size: the leading token's values, V's
+    scales unlike."""
+    p = filled(46, [700, 300], page=32, kv_heads=2, hd=64)
+    p.scale[:, :, :, :, 1] *= np.exp2(np.random.default_rng(2).integers(
+        -12, 13, p.scale[:, :, :, :, 1].shape)).astype(np.float32)
+    seqs, counts, heads = [0, 1], [3, 1], 8
+    q = (std * np.random.default_rng(8).normal(0, 1, (4, heads * 64))).astype(np.float32)
+    d = R.DevPool(dev, p)
+    for window in (0, 500):
+        got = d.attention(0, seqs, starts(counts), q, heads, window=window, max_len=700)
+        for r, (s, pos) in enumerate(((0, 697), (0, 698), (0, 699), (1, 299))):
+            k, v = p.values(s, 0)
+            lo = max(0, pos - window + 1) if window else 0
+            for h in range(heads):
+                row = q[r, 64 * h:64 * h + 64].astype(np.float64)
+                z = k[lo:pos + 1, h // 4] @ row / 8
+                best, top = np.argmax(z), np.sort(z)[-2:]
+                # a score is off by 3 e max |q| sum |k| and 10 e of itself (e = 2^-24)
+                far = 2 * 2.0 ** -24 * (10 * np.abs(z).max() + 3 * np.abs(row).max() *
+                                        np.abs(k[lo:pos + 1, h // 4]).sum(1).max() / 8)
+                # beyond that, 40 more leave others e^-40, times V's 2^24 or so: below 2^-33
+                if top[1] - top[0] < far + 40:
+                    continue
+                want = v[lo + best, h // 4]
+                # exact digits: 2^-23 of the weight, few roundings of 2^-24, exp2's 2^-22
+                assert np.abs(got[r, h] - want).max() <= 2.0 ** -20 * np.abs(want).max()
+
+
 def test_attention_of_sinks(dev):
     """A token whose score leads all others by 2^5 to 2^90, first, last or amid rounds
     of 256 others, whose values are far smaller or larger than its own."""
