@@ -618,6 +618,48 @@ def test_a_search_step_by_step_and_captured(dev):
         dev.graph_destroy(g)
 
 
+def test_parts_captured_and_replayed(dev):
+    """Calls whose work is cut into parts share the context's scratch: one after the other in
+    a graph, replayed with eager calls of other sizes between."""
+    p = filled(47, [3001, 90, 700], page=64, kv_heads=2, hd=64)
+    d = R.DevPool(dev, p)
+    rng = np.random.default_rng(3)
+    q = rng.normal(0, 1, (3, 8 * 64)).astype(np.float32)
+    x = rng.normal(0, 3, (2, 60000)).astype(np.float32)
+    seqs, start = d.list([0, 1, 2]), d.list([0, 1, 2, 3])
+    dq, dx, t = dev.upload(q), dev.upload(x), d.list([77, 59999])
+    add, none = d.list([0, 0, 0]), d.list([9])
+    outs = [dev.alloc(3 * 512 * 4), dev.alloc(8), dev.alloc(8), dev.alloc(2 * 20 * 4)]
+
+    def step():
+        dev.kv_pool_extend(d.h, seqs.ptr, add.ptr, 3, none.ptr)
+        dev.kv_pool_attention(d.h, 0, seqs.ptr, start.ptr, 3, 3, 8, dq.ptr, outs[0].ptr, max_len=3001)
+        dev.logprobs(dx.ptr, 2, 60000, t.ptr, outs[1].ptr, None, outs[2].ptr, 20, outs[3].ptr)
+
+    def results():
+        dev.sync()
+        return [dev.download(b, (n,), np.uint32) for b, n in zip(outs, (3 * 512, 2, 2, 40))]
+
+    step()
+    want = results()
+    exact = p.attention(0, [0, 1, 2], starts([1, 1, 1]), q, 8)
+    bound = R.attention_bound(p, 0, [0, 1, 2], starts([1, 1, 1]), q, 8)
+    assert (np.abs(want[0].view(np.float32).reshape(3, 8, 64) - exact) <= bound).all()
+    np.testing.assert_array_equal(want[3].view(np.int32).reshape(2, 20),
+                                  np.argsort(-x, 1, kind="stable")[:, :20])
+    g = dev.capture(step)
+    try:
+        for i in range(3):
+            dev.graph_launch(g)
+            for got, w in zip(results(), want):
+                np.testing.assert_array_equal(got, w)
+            check(d, p, [2, 0], [1 + i, 2], 8, 30 + i)
+            dev.logprobs(dx.ptr, 1, 50000 + i, t.ptr, outs[1].ptr, None, outs[2].ptr, 20, outs[3].ptr)
+            dev.sync()
+    finally:
+        dev.graph_destroy(g)
+
+
 def test_another_stream_and_context(dev):
     """Two contexts on one device, one of them on the other's stream, share a pool."""
     p = filled(40, [77, 130], page=32, kv_heads=2, hd=64)
