@@ -695,7 +695,8 @@ __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
 // round and after its last, 0.4 + 0.009 head_dim a round, 5 for a thousand workgroups, 4 for
 // joining parts; 768 workgroups at once (512 where registers allow two a CU), of
 // several sequences 0.6 of the longest's parts filled.  (702 tokens of head_dim 64: one
-// part 8.2, three 10.4; 1500 of 128: one 14.2, six 11.0; 64 sequences of up to 1024: one 15.1, four 19.4.)
+// part 8.0, three 9.6; 1500 of 128: one 15.7, six 10.7; 64 sequences of up to 1024: one 14.8, four
+// 19.0; 32 of up to 4096: eight 21.2, four 21.2, sixteen 25.9.)
 AttnArgs attn_plan(const PoolView& p, const Ragged& r, int n_heads, int max_len, int window) {
   AttnArgs a = {};
   a.p = p;

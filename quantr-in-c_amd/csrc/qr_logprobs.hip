@@ -220,7 +220,7 @@ __device__ inline void best_add(Best& b, uint32_t (&o)[16], int n, u64* buf, At 
   b.value = b.bound ? value_of(b.bound) : kNegInf;
 }
 
-// Of c keys in LDS (c <= 64 R), those that can be among the best n, one a lane in no
+// Of c keys in LDS (held in R registers a lane, c <= 64 R, or read again each time, R = 0), those that can be among the best n, one a lane in no
 // order, by one wave: a bound that at least n of them reach is raised bit by bit until 64 or
 // fewer are left.  Where it ends with more (equal logits), the 64 best in order.
 template <int R>
@@ -229,7 +229,7 @@ __device__ inline u64 choose(u64* cand, int c, int n) {
   uint32_t t = 0;
   int count = c;
   if (c > 64) {
-    uint32_t o[R];
+    uint32_t o[R > 0 ? R : 1];
 #pragma unroll
     for (int j = 0; j < R; j++)
       o[j] = 64 * j + lane < c ? (uint32_t)(cand[64 * j + lane] >> 32) : 0;
@@ -239,6 +239,9 @@ __device__ inline u64 choose(u64* cand, int c, int n) {
       int m = 0;
 #pragma unroll
       for (int j = 0; j < R; j++) m += __popcll(__ballot(o[j] >= u));
+      if (R == 0)
+        for (int i = lane; i - lane < c; i += 64)
+          m += __popcll(__ballot(i < c && (uint32_t)(cand[i] >> 32) >= u));
       if (m >= n) {
         t = u;
         count = m;
@@ -537,7 +540,7 @@ __global__ __launch_bounds__(64 * W) void k_logprobs_join(LogprobArgs a) {
     __syncthreads();
     if (wave == 0)
       key = sort64(W == 1 || count <= 512 ? choose<8>(cand, count, a.n_top)
-                                          : choose<kChoose / 64>(cand, count, a.n_top));
+                                          : choose<0>(cand, count, a.n_top));
   } else {
     __syncthreads();
   }

@@ -55,7 +55,8 @@ def check_logprobs(dev, x, V, targets, n, off=0):
 
 @pytest.mark.parametrize("rows,V,n", [(1, 1, 1), (3, 2, 5), (2, 63, 64), (1, 1023, 20), (5, 1024, 1),
                                       (2, 4097, 7), (1, 32000, 20), (3, 151936, 64), (9, 50001, 0),
-                                      (300, 5000, 3), (1100, 4200, 2)])
+                                      (300, 5000, 3), (1100, 4200, 2), (2, 600001, 20), (2, 300000, 64),
+                                      (1, 4300001, 33)])
 def test_logprobs_sizes(dev, rows, V, n):
     rng = np.random.default_rng(V + n)
     x = (rng.normal(0, 3, (rows, V + rows % 5))).astype(np.float32)
