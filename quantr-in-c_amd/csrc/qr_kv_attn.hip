@@ -360,10 +360,10 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
   for (int r = 0; r < RT; r++) qs[r] = sqs[16 * r + n];
 
   float o[RT][NV][4], M[RT], N[RT], L[RT];
-  float top[RT];  // the largest weight's power so far
+  float top[RT], tops[RT];  // the largest weight's power so far, and the largest score's
 #pragma unroll
   for (int r = 0; r < RT; r++) {
-    M[r] = N[r] = top[r] = kNone;
+    M[r] = N[r] = top[r] = tops[r] = kNone;
     L[r] = 0.0f;
 #pragma unroll
     for (int d = 0; d < NV; d++)
@@ -465,8 +465,11 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
                                  smax[3][r][n]);
       top[r] = larger(top[r], round);
       const float to = reference(larger(round, top[r] - kFall));
-      const float tos = reference(larger(larger(larger(larger(N[r], smaxs[0][r][n]),
-                                                       smaxs[1][r][n]), smaxs[2][r][n]), smaxs[3][r][n]));
+      // (of the maximum, never of the N before: a reference's own reference lies above it, and a
+      // denominator against what rises every round vanishes after 2000 of them)
+      tops[r] = larger(larger(larger(larger(tops[r], smaxs[0][r][n]), smaxs[1][r][n]), smaxs[2][r][n]),
+                       smaxs[3][r][n]);
+      const float tos = reference(tops[r]);
       const float ref = to == kNone ? 0.0f : to, refs = tos == kNone ? 0.0f : tos;
       alpha[r] = lift(M[r], ref);
       L[r] *= lift(N[r], refs);
