@@ -493,9 +493,10 @@ def _plain_pages(s):
     _count(refs, torch.where(copy, last, -1), -1)
     refs[free] = torch.where(torch.arange(N, device="cuda") < total, 1, refs[free])
     length[kids] += s["add"]
-    src, dst = torch.where(copy, last, free[0]), torch.where(copy, fresh, free[0])
-    s["data"][:, dst] = s["data"][:, src]
-    s["scale"][:, dst] = s["scale"][:, src]
+    # where nothing is copied, the page in use onto itself: no other child writes it
+    dst = torch.where(copy, fresh, last)
+    s["data"][:, dst] = s["data"][:, last]
+    s["scale"][:, dst] = s["scale"][:, last]
     s["status"].zero_()
     return _pages_out(s, status=s["status"])
 
