@@ -614,8 +614,7 @@ __global__ __launch_bounds__(256) void k_pool_store(PoolView p, Ragged r, const 
   }
 }
 
-// The same split backwards.  A slot without a page reads the layer's first
-// block, which is there, under a scale of 0.
+// The same split backwards.  A slot without a page has a block of zeros.
 template <int HD>
 __global__ __launch_bounds__(256) void k_pool_load(PoolView p, Ragged r, float* k, float* v,
                                                    long stride, int slots) {
@@ -641,7 +640,7 @@ __global__ __launch_bounds__(256) void k_pool_load(PoolView p, Ragged r, float* 
 #pragma unroll
     for (int j = 0; j < N; j++) {
       const int e = lane + 64 * j;
-      block[j] = e < kKvBlock * Q ? reinterpret_cast<const int*>(in)[e] : 0;
+      block[j] = b.there && e < kKvBlock * Q ? reinterpret_cast<const int*>(in)[e] : 0;
     }
 #pragma unroll
     for (int j = 0; j < N; j++) {
@@ -658,7 +657,7 @@ __global__ __launch_bounds__(256) void k_pool_load(PoolView p, Ragged r, float* 
     for (int j = 0; j < N; j++) {
       const int c = lane + 64 * j;
       block[j] = make_int4(0, 0, 0, 0);
-      if (c < HD) block[j] = *reinterpret_cast<const int4*>(in + c * kKvBlock);
+      if (b.there && c < HD) block[j] = *reinterpret_cast<const int4*>(in + c * kKvBlock);
     }
 #pragma unroll
     for (int j = 0; j < N; j++) {
