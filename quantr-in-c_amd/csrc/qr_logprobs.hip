@@ -220,9 +220,10 @@ __device__ inline void best_add(Best& b, uint32_t (&o)[16], int n, u64* buf, At 
   b.value = b.bound ? value_of(b.bound) : kNegInf;
 }
 
-// Of c keys in LDS (held in R registers a lane, c <= 64 R, or read again each time, R = 0), those that can be among the best n, one a lane in no
-// order, by one wave: a bound that at least n of them reach is raised bit by bit until 64 or
-// fewer are left.  Where it ends with more (equal logits), the 64 best in order.
+// Of c keys in LDS (held in R registers a lane, c <= 64 R, or read again each time, R = 0),
+// those that can be among the best n, one a lane in no order, by one wave: a bound that at
+// least n of them reach is raised bit by bit until 64 or fewer are left.  Where it ends with
+// more (equal logits), the 64 best in order.
 template <int R>
 __device__ inline u64 choose(u64* cand, int c, int n) {
   const int lane = threadIdx.x & 63;
@@ -378,19 +379,20 @@ __global__ __launch_bounds__(256, 4) void k_logprobs(LogprobArgs a) {
       }
     }
     const float m = fmaxf(s.m, mx), ref = m == kNegInf ? 0.0f : m;
-    {
-      const float d = fmaxf(s.m - ref, kFar), e = exp_of(d);
-      s.U = (s.U + s.S * d) * e;
-      s.S = s.S * e;
-      s.m = m;
-    }
+    // The segment's 16 terms first, then onto the lane's: one after the other, terms below half of
+    // the last place of a large sum would all be lost.
+    float S = 0.0f, U = 0.0f;
 #pragma unroll
     for (int j = 0; j < 16; j++) {
       const float d = __builtin_elementwise_maximum(f[j] - ref, kFar);  // keeps NaN
       const float p = exp_of(d);
-      s.S += p;
-      s.U = __builtin_fmaf(p, d, s.U);
+      S += p;
+      U = __builtin_fmaf(p, d, U);
     }
+    const float d = fmaxf(s.m - ref, kFar), e = exp_of(d);
+    s.U = __builtin_fmaf(__builtin_fmaf(s.S, d, s.U), e, U);
+    s.S = __builtin_fmaf(s.S, e, S);
+    s.m = m;
     if (RANK) {  // last: the target's logit takes two loads, one after the other
       if (target >= at && target < at + kSeg) {
 #pragma unroll
