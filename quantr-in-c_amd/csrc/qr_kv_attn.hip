@@ -1,17 +1,18 @@
 // qr_kv_attn.hip -- attention of a ragged batch over a shared 8-bit KV pool
-// (qr_kv_pool_attention), both products on int8 MFMA in fp32 accuracy.
+// (qr_kv_pool_attention), both products on MFMA.
 //
 // For a query row q and the cached k_t = ks_b kq_t, v_t = vs_b vq_t (int8
 // values, one scale per block b of 16 tokens):
 //   s_t = scale q . k_t,  out = sum_t exp(s_t) v_t / sum_t exp(s_t).
-// The cache's operands are int8 already.  The other operand of each product is
-// an fp32 number, which three int8 digits hold: x = u (65536 d2 + 256 d1 + d0),
-// d in -128 .. 127, with u chosen by the row's (q) or the tile's (weights)
-// largest value.  A product is then three exact integer products of 8 bits, and
-// what it loses is the digits' last place, 2^-23 of the largest value: no less
-// than fp32 products in fp32 sums keep.  The three products run on
-// v_mfma_i32_16x16x64_i8 at twice the rate of bf16 and read the cache's bytes
-// as they lie, so nothing is dequantized on the way.
+// Scores: q in three int8 digits, x = u (65536 d2 + 256 d1 + d0), d in -128 .. 127, with u chosen
+// by the row's largest value: three exact integer products of the cache's bytes as they lie, which
+// lose the digits' last place, 2^-24 of the row's largest value.
+// Values: the weights in two fp16 pieces, the nearest one and 2048 times what it leaves, which
+// hold a weight to 2^-22 of itself (its score's roundings move it more) or 2^-50 of the
+// largest, and V's bytes widened to fp16, 1.25 instructions each: exact products, summed in
+// fp32.  (Weights as digits of the largest, 42 us for a prompt's 512 rows, cost the others their
+// bits where one token of little value leads: beside a share of 0.9999 the rest of the output was
+// off by a fifth.  Three bf16 pieces, which know no largest, took 50 us, these 44.)
 //
 // A workgroup of four waves serves a tile of 16 or 32 rows (queries times the query
 // heads of a kv head) and takes 256 tokens a round, a wave 64 of them.  A wave's four
@@ -20,11 +21,10 @@
 //   16 g + 4 t + i; B = the rows' digits.  D then leaves row lane % 16 the four
 //   tokens 4 t .. 4 t + 3 of block g, over the four tiles all 16 of them.
 //   values: A = 16 columns of V, whose 16 bytes are a block's 16 tokens of a
-//   column; B = the digits of the weights, in the lanes and bytes where the scores
+//   column, eight to an instruction; B = the weights' pieces, in the lanes where the scores
 //   left them, so no weight crosses a lane.
 // The values' columns are what the waves share out: each reads all four waves'
-// digits from LDS (12 KiB) and sums 256 tokens in integers before anything is
-// rounded.  A wave that kept all columns of its own tokens instead converted four
+// pieces from LDS (16 KiB).  A wave that kept all columns of its own tokens instead converted four
 // times as many sums, held 206 registers for 164, and ended in a join of the waves.
 //
 // What bounds it: many rows, the issue of VALU instructions beside the matrix ones (a
@@ -35,11 +35,10 @@
 //
 // The weights carry V's scale: with vs = f 2^e (1/2 <= f < 1), w_t = f 2^(s_t
 // log2(e) + e - M) against a reference M that brings the round's largest weight just
-// below 1 (more than 2^kFall below the row's largest it does not follow), so the
-// digits are taken from the numbers that are summed and hold them to 2^-24 of the largest
-// of 256.  The denominator runs against the maximum N of the scores alone, its
-// terms the same powers times 2^(M - e - N): values of V however unlike move no token out
-// of it.
+// below 1 (more than 2^kFall below the row's largest it does not follow), so the pieces are
+// those of the numbers that are summed.  The denominator runs against the maximum N of the scores
+// alone, its terms the same powers times 2^(M - e - N): values of V however unlike move no
+// token out of it.
 #include <math.h>
 
 #include "qr_kv_pool.h"
@@ -49,6 +48,10 @@ namespace qr {
 namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kStep = 64;   // tokens of a wave's step
 constexpr int kWaves = 4;   // of a workgroup
@@ -58,11 +61,8 @@ constexpr int kMaxParts = 1024;  // of a tile's tokens
 constexpr long kMostItems = 32768;  // workgroups with parts: what they leave stays below 600 MB
 constexpr int kJoinWave = 16;    // up to as many one wave joins a row
 constexpr float kNone = -INFINITY;
-// Weights up to 1 become whole numbers below 2^23 - 0x8080: added to 2^23 +
-// 0x8080 they are the low mantissa bits of a float, and its three low bytes the
-// digits but for the 0x80 that the two lower bytes carry.
-constexpr float kWMul = 8355600.0f;
-constexpr float kWAdd = 8388608.0f + 32896.0f;
+// A number up to kTop as two fp16: the nearest one, and kSecond times what it leaves.
+constexpr float kTop = 32768.0f, kSecond = 2048.0f;
 constexpr float kQMax = 8355711.0f;  // 127 * (65536 + 256 + 1)
 // Exponent of V scales that are 0 or smaller than it: such a block's weights
 // lead no others.
@@ -162,10 +162,30 @@ __device__ inline v4i mfma(v4i a, v4i b, v4i c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
-// 65536 d2 + 256 d1 + d0 of three products, rounded to fp32 (the first two sum
-// up below 2^31 over 64 tokens or 256 columns).
+// 65536 d2 + 256 d1 + d0 of three products, rounded to fp32 (the first two sum up below
+// 256 * 256 * 128 * 128 + 2^22 < 2^31 over 256 columns).
 __device__ inline float joined(int s2, int s1, int s0) {
   return __builtin_fmaf((float)(s2 * 256 + s1), 256.0f, (float)s0);
+}
+
+// Two numbers' pieces: a = p0 + p1 / kSecond to 2^-22 of a, or 2^-36 where that is more.
+__device__ inline void pieces2(float a, float b, int* p0, int* p1) {
+  const v2h h = __builtin_convertvector((v2f{a, b}), v2h);
+  const v2f left = {__builtin_fmaf(-kSecond, (float)h.x, a * kSecond),
+                    __builtin_fmaf(-kSecond, (float)h.y, b * kSecond)};
+  *p0 = __builtin_bit_cast(int, h);
+  *p1 = __builtin_bit_cast(int, __builtin_convertvector(left, v2h));
+}
+
+// Eight int8 as fp16, exactly: beside the byte 0x64 the unsigned x + 128 is the fp16 1024 + 128 + x.
+__device__ inline v8h widened(int lo, int hi) {
+  const uint32_t a = (uint32_t)lo ^ 0x80808080u, b = (uint32_t)hi ^ 0x80808080u;
+  const v4i w = {(int)perm(0x64646464u, a, 0x05010400u), (int)perm(0x64646464u, a, 0x07030602u),
+                 (int)perm(0x64646464u, b, 0x05010400u), (int)perm(0x64646464u, b, 0x07030602u)};
+  return __builtin_bit_cast(v8h, w) - (_Float16)1152.0f;
+}
+__device__ inline v4f mfma(v8h a, int4 b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
 __device__ inline int4 load16(const int8_t* p) { return *reinterpret_cast<const int4*>(p); }
@@ -188,14 +208,14 @@ __device__ inline float lift(float m, float to) {
 // What a sum against M is multiplied by for the result, with the denominator l
 // against N; 0 for a row that saw nothing.
 __device__ inline float over(float M, float N, float l) {
-  return l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(M - N) / (l * kWMul);
+  return l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(M - N) / (l * kTop);
 }
 
 template <int HD, int RT>
 __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) void k_pool_attn(AttnArgs a) {
   constexpr int NC = (HD + 63) / 64;            // 64-column chunks of a K row
   constexpr int NV = (HD / 16 + 3) / kWaves;    // 16-column tiles of V for a wave
-  __shared__ int4 sp[kWaves][RT][3][64];        // the weights' digits
+  __shared__ int4 sp[kWaves][RT][2][2][64];     // the weights' pieces, eight tokens each
   __shared__ __align__(16) int8_t sq[3][16 * RT][NC * 64 + 16];  // the rows' digits
   __shared__ float sqs[16 * RT];                   // and what one of the last place stands for
   __shared__ int spg[kPages];
@@ -388,7 +408,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
         ev = __builtin_amdgcn_frexp_expf(vs);
         f = __builtin_amdgcn_frexp_mantf(vs);
       }
-      fw = f * kWMul;
+      fw = f * kTop;
       lf = fmaxf(__builtin_amdgcn_logf(f), -1.0f);
       evf = (float)ev;
       // Every token of the step seen by every row of the tile?
@@ -481,58 +501,77 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
         const float base = ref - deep, down = ref - base;
         const float fwd = __builtin_ldexpf(fw, -(int)down);
         float sum = 0.0f;
-        int4 p[3];
-        int* d0 = &p[0].x;
-        int* d1 = &p[1].x;
-        int* d2 = &p[2].x;
+        int4 p[2][2];
 #pragma unroll
         for (int tt = 0; tt < 4; tt++) {
-          uint32_t u[4];
+          float w[4];
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const float w = __builtin_amdgcn_exp2f(e[r][4 * tt + i] - base);
-            sum += w;
-            u[i] = __builtin_bit_cast(uint32_t, __builtin_fmaf(w, fwd, kWAdd));
+            const float x = __builtin_amdgcn_exp2f(e[r][4 * tt + i] - base);
+            sum += x;
+            w[i] = x * fwd;
           }
-          digits4(u[0], u[1], u[2], u[3], d0 + tt, d1 + tt, d2 + tt);
+          const int at = 2 * (tt & 1), h = tt >> 1;
+          pieces2(w[0], w[1], &p[0][h].x + at, &p[1][h].x + at);
+          pieces2(w[2], w[3], &p[0][h].x + at + 1, &p[1][h].x + at + 1);
         }
         L[r] = __builtin_fmaf(sum, __builtin_amdgcn_exp2f((ref - refs) - down - evf), L[r]);
 #pragma unroll
-        for (int k = 0; k < 3; k++) sp[wave][r][k][lane] = p[k];
-      } else {
-        // no tokens: digits of 0, whatever V holds there
+        for (int k = 0; k < 2; k++)
 #pragma unroll
-        for (int k = 0; k < 3; k++) sp[wave][r][k][lane] = make_int4(0, 0, 0, 0);
+          for (int h = 0; h < 2; h++) sp[wave][r][k][h][lane] = p[k][h];
+      } else {
+        // no tokens: weights of 0, whatever V holds there
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) sp[wave][r][k][h][lane] = make_int4(0, 0, 0, 0);
       }
     }
     __syncthreads();
     __builtin_amdgcn_s_setprio(1);
-    // Values: 256 tokens in integers (below 2^22, 2^30 with the next digit).
+    // Values of 256 tokens, each piece's apart; in two chains where there are few.
+    constexpr int kChains = RT * NV < 4 ? 2 : 1;
+    v4f acc[RT][NV][kChains][2];
 #pragma unroll
-    for (int r = 0; r < RT; r++) {
-      v4i acc[NV][3];
+    for (int r = 0; r < RT; r++)
 #pragma unroll
       for (int d = 0; d < NV; d++)
 #pragma unroll
-        for (int k = 0; k < 3; k++) acc[d][k] = v4i{0, 0, 0, 0};
+        for (int j = 0; j < kChains; j++) acc[r][d][j][0] = acc[r][d][j][1] = v4f{0, 0, 0, 0};
 #pragma unroll
-      for (int s = 0; s < kWaves; s++) {
-        v4i w[3];
+    for (int s = 0; s < kWaves; s++)
 #pragma unroll
-        for (int k = 0; k < 3; k++) w[k] = as_v4(sp[s][r][k][lane]);
+      for (int h = 0; h < 2; h++) {
+        const int j = h % kChains;
+        int4 w[RT][2];
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+          for (int k = 0; k < 2; k++) w[r][k] = sp[s][r][k][h][lane];
 #pragma unroll
         for (int d = 0; d < NV; d++)
-          if (HD % 64 == 0 || wave + 4 * d < HD / 16)
+          if (HD % 64 == 0 || wave + 4 * d < HD / 16) {
+            const v8h v = h ? widened(vr[d][s].z, vr[d][s].w) : widened(vr[d][s].x, vr[d][s].y);
 #pragma unroll
-            for (int k = 0; k < 3; k++) acc[d][k] = mfma(as_v4(vr[d][s]), w[k], acc[d][k]);
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+              for (int k = 0; k < 2; k++) acc[r][d][j][k] = mfma(v, w[r][k], acc[r][d][j][k]);
+          }
       }
+#pragma unroll
+    for (int r = 0; r < RT; r++)
 #pragma unroll
       for (int d = 0; d < NV; d++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          o[r][d][i] =
-              __builtin_fmaf(o[r][d][i], alpha[r], joined(acc[d][2][i], acc[d][1][i], acc[d][0][i]));
-    }
+        for (int i = 0; i < 4; i++) {
+          float hi = acc[r][d][0][0][i], lo = acc[r][d][0][1][i];
+          if (kChains == 2) {
+            hi += acc[r][d][kChains - 1][0][i];
+            lo += acc[r][d][kChains - 1][1][i];
+          }
+          o[r][d][i] = __builtin_fmaf(o[r][d][i], alpha[r], __builtin_fmaf(lo, 1.0f / kSecond, hi));
+        }
     __builtin_amdgcn_s_setprio(0);
   }
 
