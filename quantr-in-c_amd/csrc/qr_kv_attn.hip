@@ -4,22 +4,23 @@
 // For a query row q and the cached k_t = ks_b kq_t, v_t = vs_b vq_t (int8
 // values, one scale per block b of 16 tokens):
 //   s_t = scale q . k_t,  out = sum_t exp(s_t) v_t / sum_t exp(s_t).
-// Scores: q in three int8 digits, x = u (65536 d2 + 256 d1 + d0), d in -128 .. 127, with u chosen
-// by the row's largest value: three exact integer products of the cache's bytes as they lie, which
-// lose the digits' last place, 2^-24 of the row's largest value.
-// Values: the weights in two fp16 pieces, the nearest one and 2048 times what it leaves, which
-// hold a weight to 2^-22 of itself (its score's roundings move it more) or 2^-50 of the
-// largest, and V's bytes widened to fp16, 1.25 instructions each: exact products, summed in
-// fp32.  (Weights as digits of the largest, 42 us for a prompt's 512 rows, cost the others their
-// bits where one token of little value leads: beside a share of 0.9999 the rest of the output was
-// off by a fifth.  Three bf16 pieces, which know no largest, took 50 us, these 44.)
+// The other operand of each product is an fp32 number, a row's q or a token's weight: two fp16
+// pieces, the nearest one and 2048 times what it leaves, hold it to 2^-22 of itself (a
+// score's own roundings in fp32 move a weight more) or 2^-50 of the largest of its row (q) or of 256
+// tokens (weights).  The cache's bytes are widened to fp16 on the way, 1.25 instructions
+// each; products are exact and sums fp32, each piece's apart.  (Digits of the largest on int8
+// products, 40 us for a prompt's 512 rows where this takes 48, gave the small ones up: beside a token
+// that takes 0.9999 of the weight with values of 0 the output was off by a fifth of itself,
+// beside a channel of q of 10^6 by a fortieth.  Three bf16 pieces of the weights, which know no
+// largest, took 50 us where two of fp16 took 44.)
 //
 // A workgroup of four waves serves a tile of 16 or 32 rows (queries times the query
 // heads of a kv head) and takes 256 tokens a round, a wave 64 of them.  A wave's four
 // lane groups g = lane / 16 own a block each:
 //   scores: A = 16 tokens of K in four tiles, tile t's row 4 g + i being token
-//   16 g + 4 t + i; B = the rows' digits.  D then leaves row lane % 16 the four
-//   tokens 4 t .. 4 t + 3 of block g, over the four tiles all 16 of them.
+//   16 g + 4 t + i, eight of a lane's 16 columns to an instruction; B = the rows' pieces.  D
+//   then leaves row lane % 16 the four tokens 4 t .. 4 t + 3 of block g, over the four tiles
+//   all 16 of them.
 //   values: A = 16 columns of V, whose 16 bytes are a block's 16 tokens of a
 //   column, eight to an instruction; B = the weights' pieces, in the lanes where the scores
 //   left them, so no weight crosses a lane.
@@ -63,7 +64,6 @@ constexpr int kJoinWave = 16;    // up to as many one wave joins a row
 constexpr float kNone = -INFINITY;
 // A number up to kTop as two fp16: the nearest one, and kSecond times what it leaves.
 constexpr float kTop = 32768.0f, kSecond = 2048.0f;
-constexpr float kQMax = 8355711.0f;  // 127 * (65536 + 256 + 1)
 // Exponent of V scales that are 0 or smaller than it: such a block's weights
 // lead no others.
 constexpr int kMinExp = -60;
@@ -148,26 +148,6 @@ __device__ inline uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
   return __builtin_amdgcn_perm(hi, lo, sel);
 }
 
-// Four numbers whose bytes 0 and 1 carry 0x80 -> their digits, four to a dword.
-__device__ inline void digits4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int* d0, int* d1,
-                               int* d2) {
-  const uint32_t lo = perm(b, a, 0x05010400u), hi = perm(d, c, 0x05010400u);
-  *d0 = (int)(perm(hi, lo, 0x05040100u) ^ 0x80808080u);
-  *d1 = (int)(perm(hi, lo, 0x07060302u) ^ 0x80808080u);
-  const uint32_t l2 = perm(b, a, 0x0c0c0602u), h2 = perm(d, c, 0x0c0c0602u);
-  *d2 = (int)perm(h2, l2, 0x05040100u);
-}
-
-__device__ inline v4i mfma(v4i a, v4i b, v4i c) {
-  return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
-}
-
-// 65536 d2 + 256 d1 + d0 of three products, rounded to fp32 (the first two sum up below
-// 256 * 256 * 128 * 128 + 2^22 < 2^31 over 256 columns).
-__device__ inline float joined(int s2, int s1, int s0) {
-  return __builtin_fmaf((float)(s2 * 256 + s1), 256.0f, (float)s0);
-}
-
 // Two numbers' pieces: a = p0 + p1 / kSecond to 2^-22 of a, or 2^-36 where that is more.
 __device__ inline void pieces2(float a, float b, int* p0, int* p1) {
   const v2h h = __builtin_convertvector((v2f{a, b}), v2h);
@@ -184,12 +164,11 @@ __device__ inline v8h widened(int lo, int hi) {
                  (int)perm(0x64646464u, b, 0x05010400u), (int)perm(0x64646464u, b, 0x07030602u)};
   return __builtin_bit_cast(v8h, w) - (_Float16)1152.0f;
 }
-__device__ inline v4f mfma(v8h a, int4 b, v4f c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+__device__ inline v4f mfma(v8h a, v8h b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
 __device__ inline int4 load16(const int8_t* p) { return *reinterpret_cast<const int4*>(p); }
-__device__ inline v4i as_v4(int4 x) { return v4i{x.x, x.y, x.z, x.w}; }
 
 // The reference for weights up to 2^x: the next multiple of 1 / 16, so that the references'
 // and V's exponents differ by what fp32 holds exactly and no rounding of theirs moves a
@@ -216,8 +195,8 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
   constexpr int NC = (HD + 63) / 64;            // 64-column chunks of a K row
   constexpr int NV = (HD / 16 + 3) / kWaves;    // 16-column tiles of V for a wave
   __shared__ int4 sp[kWaves][RT][2][2][64];     // the weights' pieces, eight tokens each
-  __shared__ __align__(16) int8_t sq[3][16 * RT][NC * 64 + 16];  // the rows' digits
-  __shared__ float sqs[16 * RT];                   // and what one of the last place stands for
+  __shared__ __align__(16) _Float16 sq[2][16 * RT][NC * 64 + 8];  // the rows' pieces
+  __shared__ float sqs[16 * RT];                   // and what they are multiplied by
   __shared__ int spg[kPages];
   __shared__ float smax[kWaves][RT][16], smaxs[kWaves][RT][16];
   __shared__ float ssum[kWaves][RT][16];
@@ -310,7 +289,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     for (int tt = 0; tt < 4; tt++)
 #pragma unroll
       for (int c = 0; c < NC; c++)
-        // columns behind the row: the lane's first ones again, against digits of 0
+        // columns behind the row: the lane's first ones again, against a q of 0
         kr[tt][c] = load16(s + 4 * tt * HD + (HD % 64 == 0 || 64 * c + 16 * g < HD ? 64 * c : 0));
     here = wp >= 0;
     sc = make_float2(0.0f, 0.0f);
@@ -336,7 +315,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     load_k(tb);
   }
 
-  // q's digits, for all waves
+  // q's pieces, for all waves: times a power of two that brings the row's largest to 2^14 .. 2^15
 #pragma unroll
   for (int i = 0; i < kTurns; i++) {
     const int at = (i * kWaves + wave) * kSets + lane / kPer;
@@ -358,21 +337,16 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
       amax = fmaxf(amax, lane_xor_f<32>(amax));
       bad = fmaxf(bad, lane_xor_f<32>(bad));
     }
-    // a row below 2^-96 is held to 2^-119
-    amax = fmaxf(amax, 1.2621774e-29f);
-    const float inv = kQMax / amax;
-    uint32_t u[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      u[j] = (uint32_t)((int)rintf(fminf(fmaxf(v[j] * inv, -kQMax), kQMax)) + 0x8080);
-    int e0, e1, e2;
-    digits4(u[0], u[1], u[2], u[3], &e0, &e1, &e2);
+    // (a row below 2^-96 less far: the factor that takes it back stays a normal number)
+    const int e = 15 - __builtin_amdgcn_frexp_expf(amax), up = e < 111 ? e : 111;
+    int2 p0, p1;
+    pieces2(__builtin_ldexpf(v[0], up), __builtin_ldexpf(v[1], up), &p0.x, &p1.x);
+    pieces2(__builtin_ldexpf(v[2], up), __builtin_ldexpf(v[3], up), &p0.y, &p1.y);
     if (qc < NC * 64) {
-      *reinterpret_cast<int*>(&sq[0][at][qc]) = e0;
-      *reinterpret_cast<int*>(&sq[1][at][qc]) = e1;
-      *reinterpret_cast<int*>(&sq[2][at][qc]) = e2;
+      *reinterpret_cast<int2*>(&sq[0][at][qc]) = p0;
+      *reinterpret_cast<int2*>(&sq[1][at][qc]) = p1;
     }
-    if (qc == 0) sqs[at] = bad > 0.0f ? NAN : amax / kQMax * a.scale2;
+    if (qc == 0) sqs[at] = bad > 0.0f ? NAN : __builtin_ldexpf(a.scale2, -up);
   }
   __syncthreads();
   float qs[RT];
@@ -414,29 +388,40 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
       // Every token of the step seen by every row of the tile?
       const bool full = __all(here) && Tw + kStep <= t.pos0 + 1 &&
                         (a.window == 0 || Tw >= t.pos0 + t.queries - a.window);
+      v8h qd[RT][NC][2][2];
 #pragma unroll
-      for (int r = 0; r < RT; r++) {
-        const float c = qs[r] * sc.x;
-        v4i qd[NC][3];
+      for (int r = 0; r < RT; r++)
 #pragma unroll
         for (int k = 0; k < NC; k++)
 #pragma unroll
-          for (int i = 0; i < 3; i++)
-            qd[k][i] = as_v4(load16(&sq[i][16 * r + n][64 * k + 16 * g]));
+          for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int tt = 0; tt < 4; tt++) {
-          v4i s0 = {0, 0, 0, 0}, s1 = s0, s2 = s0;
+            for (int i = 0; i < 2; i++)
+              qd[r][k][h][i] = *reinterpret_cast<const v8h*>(&sq[i][16 * r + n][64 * k + 16 * g + 8 * h]);
 #pragma unroll
-          for (int k = 0; k < NC; k++) {
-            const v4i kk = as_v4(kr[tt][k]);
-            s0 = mfma(kk, qd[k][0], s0);
-            s1 = mfma(kk, qd[k][1], s1);
-            s2 = mfma(kk, qd[k][2], s2);
+      for (int tt = 0; tt < 4; tt++) {
+        v4f acc[RT][2];
+#pragma unroll
+        for (int r = 0; r < RT; r++) acc[r][0] = acc[r][1] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < NC; k++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const v8h kk = h ? widened(kr[tt][k].z, kr[tt][k].w) : widened(kr[tt][k].x, kr[tt][k].y);
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+              for (int i = 0; i < 2; i++) acc[r][i] = mfma(kk, qd[r][k][h][i], acc[r][i]);
           }
 #pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
           for (int i = 0; i < 4; i++)
-            e[r][4 * tt + i] = __builtin_fmaf(joined(s2[i], s1[i], s0[i]), c, evf);
-        }
+            e[r][4 * tt + i] = __builtin_fmaf(
+                __builtin_fmaf(acc[r][1][i], 1.0f / kSecond, acc[r][0][i]), qs[r] * sc.x, evf);
+      }
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
         if (!full) {
           const int first = row_lo[r] - (Tw + 16 * g);
           const unsigned seen = here ? row_hi[r] - row_lo[r] : 0;
@@ -544,11 +529,11 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const int j = h % kChains;
-        int4 w[RT][2];
+        v8h w[RT][2];
 #pragma unroll
         for (int r = 0; r < RT; r++)
 #pragma unroll
-          for (int k = 0; k < 2; k++) w[r][k] = sp[s][r][k][h][lane];
+          for (int k = 0; k < 2; k++) w[r][k] = __builtin_bit_cast(v8h, sp[s][r][k][h][lane]);
 #pragma unroll
         for (int d = 0; d < NV; d++)
           if (HD % 64 == 0 || wave + 4 * d < HD / 16) {

@@ -134,3 +134,28 @@ def test_sinks_of_small_values_in_ordinary_blocks(dev, hd, rows, own):
                 lo, hi = (c, hi) if w[at] / w.sum() < share else (lo, c)
             assert abs(w[at] / w.sum() - share) < 1e-6 * share
             check(d, p, [0], [rows], q, heads, scale=float(np.float32(c)), max_len=n)
+
+
+@pytest.mark.parametrize("hd,rows", [(64, 1), (64, 40), (128, 3), (128, 40), (32, 2), (96, 1), (160, 2),
+                                     (256, 5)])
+@pytest.mark.parametrize("size", [60.0, 1e4, 1e6])
+def test_outlier_channels_of_q(dev, hd, rows, size):
+    """A channel of q far above the others where K is small or 0: the others count all the same."""
+    n, heads = 500, 2
+    rng = np.random.default_rng(hd + rows)
+    p = pool_with(hd, n, hd)
+    for j, least in ((hd - 1, 0), (5, 0), (17, 1 if size < 100 else 0)):
+        for t in range(n):
+            token(p, t, 0)[j] = least * rng.integers(-1, 2)
+    q = rng.normal(0, 1.5, (rows, heads * hd)).astype(np.float32)
+    for h in range(heads):
+        q[:, h * hd + rng.choice([hd - 1, 5, 17])] = size * rng.choice([-1, 1], rows)
+    check(R.DevPool(dev, p), p, [0], [rows], q, heads, max_len=n)
+
+
+def test_ordinary_rows_to_the_same_bound(dev):
+    for hd, heads, rows, n in ((64, 8, 1, 702), (128, 8, 64, 900), (96, 4, 5, 300), (192, 1, 2, 150)):
+        p = pool_with(hd + 1, n, hd)
+        q = np.random.default_rng(n).normal(0, 1.5, (rows, heads * hd)).astype(np.float32)
+        check(R.DevPool(dev, p), p, [0], [rows], q, heads, max_len=n)
+        check(R.DevPool(dev, p), p, [0], [rows], q, heads, max_len=n, window=77)
