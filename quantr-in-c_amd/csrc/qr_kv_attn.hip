@@ -190,8 +190,10 @@ __device__ inline float over(float M, float N, float l) {
   return l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(M - N) / (l * kTop);
 }
 
+// Workgroups a CU: three of 16 rows up to head_dim 128, two otherwise; none spills (attn_plan
+// counts on as many).
 template <int HD, int RT>
-__global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) void k_pool_attn(AttnArgs a) {
+__global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : 2) void k_pool_attn(AttnArgs a) {
   constexpr int NC = (HD + 63) / 64;            // 64-column chunks of a K row
   constexpr int NV = (HD / 16 + 3) / kWaves;    // 16-column tiles of V for a wave
   __shared__ int4 sp[kWaves][RT][2][2][64];     // the weights' pieces, eight tokens each
@@ -296,6 +298,13 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     if (here)
       sc = reinterpret_cast<const float2*>(a.p.scale)[block(wp, b0 + 4 * wave + g)];
   };
+  // A tile behind the last is an earlier one again and never stored: a branch around it in the
+  // loop cost head_dim 96 18 spilled registers (4 x 1000 tokens 18.9 us, 14.3 without) and
+  // 224 its second workgroup (32 x 1500: 26.9 us, 17.1).
+  int vtile[NV];
+#pragma unroll
+  for (int d = 0; d < NV; d++)
+    vtile[d] = HD % 64 == 0 || wave + 4 * d < HD / 16 ? wave + 4 * d : wave % (HD / 16);
   auto load_v = [&](int T0) {
 #pragma unroll
     for (int s = 0; s < kWaves; s++) {
@@ -303,8 +312,7 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
                         kKvBlock * HD + n * kKvBlock;
 #pragma unroll
       for (int d = 0; d < NV; d++)
-        if (HD % 64 == 0 || wave + 4 * d < HD / 16)
-          vr[d][s] = load16(v + (wave + 4 * d) * 16 * kKvBlock);
+        vr[d][s] = load16(v + vtile[d] * 16 * kKvBlock);
     }
   };
   if (tb < te) {
@@ -515,8 +523,8 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
     }
     __syncthreads();
     __builtin_amdgcn_s_setprio(1);
-    // Values of 256 tokens, each piece's apart; in two chains where there are few.
-    constexpr int kChains = RT * NV < 4 ? 2 : 1;
+    // Values of 256 tokens, each piece's apart; in two chains where there is one tile.
+    constexpr int kChains = RT * NV < 2 ? 2 : 1;
     v4f acc[RT][NV][kChains][2];
 #pragma unroll
     for (int r = 0; r < RT; r++)
@@ -535,14 +543,13 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : HD <= 192 ? 2 : 1) 
 #pragma unroll
           for (int k = 0; k < 2; k++) w[r][k] = __builtin_bit_cast(v8h, sp[s][r][k][h][lane]);
 #pragma unroll
-        for (int d = 0; d < NV; d++)
-          if (HD % 64 == 0 || wave + 4 * d < HD / 16) {
-            const v8h v = h ? widened(vr[d][s].z, vr[d][s].w) : widened(vr[d][s].x, vr[d][s].y);
+        for (int d = 0; d < NV; d++) {
+          const v8h v = h ? widened(vr[d][s].z, vr[d][s].w) : widened(vr[d][s].x, vr[d][s].y);
 #pragma unroll
-            for (int r = 0; r < RT; r++)
+          for (int r = 0; r < RT; r++)
 #pragma unroll
-              for (int k = 0; k < 2; k++) acc[r][d][j][k] = mfma(v, w[r][k], acc[r][d][j][k]);
-          }
+            for (int k = 0; k < 2; k++) acc[r][d][j][k] = mfma(v, w[r][k], acc[r][d][j][k]);
+        }
       }
 #pragma unroll
     for (int r = 0; r < RT; r++)
