@@ -725,12 +725,13 @@ __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
 // How the work is cut.  Heads: at most 16 of a kv head's query heads share a
 // tile, as many queries beside each other as fill it; 32 rows where sequences bring
 // as many.  Tokens: a tile's part is one workgroup.  The number of rounds of a part is the
-// one with the least time by what was measured (us): 3.5 before a workgroup's first
-// round and after its last, 0.4 + 0.009 head_dim a round, 5 for a thousand workgroups, 4 for
+// one with the least time by what was measured (us): 4.5 before a workgroup's first
+// round and after its last, 0.7 + 0.014 head_dim a round, 5 for a thousand workgroups, 4 for
 // joining parts; 768 workgroups at once (512 where registers allow two a CU), of
-// several sequences 0.6 of the longest's parts filled.  (702 tokens of head_dim 64: one
-// part 8.0, three 9.6; 1500 of 128: one 15.7, six 10.7; 64 sequences of up to 1024: one 14.8, four
-// 19.0; 32 of up to 4096: eight 21.2, four 21.2, sixteen 25.9.)
+// several sequences 0.6 of the longest's parts filled.  (702 tokens of head_dim 64: one part 9.2,
+// three 9.6; 1500 of 128: one 19.7, six 11.3; 16 sequences of up to 1024: one 15.0, four 12.1; 64 of them:
+// one 17.2, four 19.3; 32 of up to 4096: eight 23.8, four 24.3, sixteen 27.9; 8 of up to 2000 of
+// head_dim 256: eight 14.2, four 18.5.)
 AttnArgs attn_plan(const PoolView& p, const Ragged& r, int n_heads, int max_len, int window) {
   AttnArgs a = {};
   a.p = p;
@@ -762,7 +763,7 @@ AttnArgs attn_plan(const PoolView& p, const Ragged& r, int n_heads, int max_len,
       const float wgs = (float)tiles * (float)parts;
       const float turns = parts > 1 ? wgs * filled / at_once : wgs / at_once;
       const float us = (turns > 1.0f ? turns : 1.0f) *
-                           (3.5f + (0.4f + 0.009f * (float)p.hd) * (float)rounds) +
+                           (4.5f + (0.7f + 0.014f * (float)p.hd) * (float)rounds) +
                        0.005f * wgs + (parts > 1 ? 4.0f : 0.0f);
       if (us < best) {
         best = us;
