@@ -64,9 +64,8 @@ constexpr int kJoinWave = 16;    // up to as many one wave joins a row
 constexpr float kNone = -INFINITY;
 // A number up to kTop as two fp16: the nearest one, and kSecond times what it leaves.
 constexpr float kTop = 32768.0f, kSecond = 2048.0f;
-// Exponent of V scales that are 0 or smaller than it: such a block's weights
-// lead no others.
-constexpr int kMinExp = -60;
+// Exponent of V scales that are 0 or subnormal: such a block's weights lead no others.
+constexpr int kMinExp = -125;
 // A block whose exponents lie further below M takes its powers 2^-kDeep below them, so that
 // they are there for the denominator.
 constexpr float kDeep = 60.0f;
@@ -184,11 +183,18 @@ __device__ inline float lift(float m, float to) {
   return m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
 }
 
-// What a sum against M is multiplied by for the result, with the denominator l
-// against N; 0 for a row that saw nothing.
-__device__ inline float over(float M, float N, float l) {
-  return l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(M - N) / (l * kTop);
-}
+// A sum against M over the denominator l against N; 0 for a row that saw nothing.  The whole
+// powers of two come last, so that nothing on the way leaves the normal numbers.
+struct Over {
+  float inv;
+  int exp;
+  __device__ Over(float M, float N, float l) {
+    const float d = M - N, whole = floorf(d);
+    exp = (int)whole;
+    inv = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(d - whole) / (l * kTop);
+  }
+  __device__ float operator()(float x) const { return __builtin_ldexpf(x * inv, exp); }
+};
 
 // Workgroups a CU: three of 16 rows up to head_dim 128, two otherwise; none spills (attn_plan
 // counts on as many).
@@ -385,8 +391,8 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : 2) void k_pool_attn
       // Exponents: scores in powers of two, with V's.
       const float vs = sc.y;
       int ev = kMinExp;
-      float f = vs * 0x1p60f;
-      if (vs > 0x1p-60f) {
+      float f = vs * 0x1p125f;
+      if (vs >= 0x1p-126f) {
         ev = __builtin_amdgcn_frexp_expf(vs);
         f = __builtin_amdgcn_frexp_mantf(vs);
       }
@@ -579,13 +585,13 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : 2) void k_pool_attn
     if (!row_ok[r]) continue;
     const float l = (ssum[0][r][n] + ssum[1][r][n]) + (ssum[2][r][n] + ssum[3][r][n]);
     if (a.splits == 1) {
-      const float inv = over(M[r], N[r], l);
+      const Over over(M[r], N[r], l);
       float* dst = a.out + row[r] * a.out_stride + (long)head[r] * HD + 4 * g;
 #pragma unroll
       for (int d = 0; d < NV; d++)
         if (HD % 64 == 0 || wave + 4 * d < HD / 16)
           *reinterpret_cast<float4*>(dst + 16 * (wave + 4 * d)) = make_float4(
-              o[r][d][0] * inv, o[r][d][1] * inv, o[r][d][2] * inv, o[r][d][3] * inv);
+              over(o[r][d][0]), over(o[r][d][1]), over(o[r][d][2]), over(o[r][d][3]));
     } else {
       const size_t at =
           ((size_t)(slot * gridDim.y + hy) * a.splits + z) * (16 * RT) + 16 * r + n;
@@ -698,7 +704,7 @@ __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
     }
   }
   float* dst = a.out + (long)(meta.x + qi) * a.out_stride + (long)(hy / a.hgroups * a.group + hh) * HD;
-  const float inv = over(M, N, L);
+  const Over over(M, N, L);
   if (W == 1) {
     float4 r = o;
 #pragma unroll
@@ -710,14 +716,14 @@ __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
     }
     if (tid < Q)
       *reinterpret_cast<float4*>(dst + 4 * c) =
-          make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
+          make_float4(over(r.x), over(r.y), over(r.z), over(r.w));
   } else {
     if (grp < G) *reinterpret_cast<float4*>(&sums[grp][4 * c]) = o;
     __syncthreads();
     if (tid < HD) {
       float sum = 0.0f;
       for (int j = 0; j < G; j++) sum += sums[j][tid];
-      dst[tid] = sum * inv;
+      dst[tid] = over(sum);
     }
   }
 }

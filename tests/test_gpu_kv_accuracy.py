@@ -42,7 +42,8 @@ def fp32_bound(p, layer, seqs, start, q, n_heads, window=0, scale=0.0):
     Both products sum exact products of two fp16 pieces of an fp32 number with int8, 32 to a matrix
     instruction, whose sum is off by at most 10 e of its largest term or of what it adds to (probed:
     7.4), the second pieces adding less than a tenth: a score by dz = 11 e c (hd / 32) sum |q_j k_tj|,
-    and by 10 e |z| + 64 e of its exponent's roundings; its weight by that and exp2's 2^-22.
+    and by 10 e |z| + (4 + |ev|) e of its exponent's roundings, V's 2^ev in it; its weight by that and
+    exp2's 2^-22.
     A value's sums take 8 such instructions for 256 tokens and a rounding for each 256: (82 + n / 256) e of
     sum w |v|; the denominator (n / 64 + 40) e of itself, the quotient 3 e.
     The pieces: the nearest fp16 leaves half of 2^-10 of a number, 2048 times that is held to half
@@ -59,6 +60,7 @@ def fp32_bound(p, layer, seqs, start, q, n_heads, window=0, scale=0.0):
         vs = np.array([[p.scale[layer, p.table[s, t // p.page], h, t % p.page // 16, 1]
                         for h in range(p.kv_heads)] for t in range(n)], np.float64)
         vq = v / vs[:, :, None]
+        ev = np.abs(np.log2(vs)) + 1
         for r in range(m):
             pos = n - m + r
             lo = max(0, pos - window + 1) if window else 0
@@ -69,7 +71,7 @@ def fp32_bound(p, layer, seqs, start, q, n_heads, window=0, scale=0.0):
                 z = kk @ row * c
                 d = (11 * e * steps + 2.0 ** -22) * c * (np.abs(kk) @ np.abs(row))
                 d += 2.0 ** -50 * c * np.abs(row).max() * np.abs(kk).sum(1)
-                d += 10 * e * np.abs(z) + 64 * e + 2.0 ** -22
+                d += 10 * e * np.abs(z) + (4 + ev[lo:pos + 1, kh]) * e + 2.0 ** -22
                 w = np.exp(z - z.max())
                 L = w.sum()
                 least = 2.0 ** -50 * (w * vs[lo:pos + 1, kh]).max()
@@ -159,3 +161,13 @@ def test_ordinary_rows_to_the_same_bound(dev):
         q = np.random.default_rng(n).normal(0, 1.5, (rows, heads * hd)).astype(np.float32)
         check(R.DevPool(dev, p), p, [0], [rows], q, heads, max_len=n)
         check(R.DevPool(dev, p), p, [0], [rows], q, heads, max_len=n, window=77)
+
+
+@pytest.mark.parametrize("size", [1e-37, 1e-33, 1e-30, 1e-25, 1e-20, 1e-10, 1e10, 1e20, 1e30, 1e35])
+def test_values_of_any_size(dev, size):
+    """V small or large everywhere, down to the least normal scales: held as well as ordinary ones."""
+    for hd, heads, rows, n in ((64, 8, 1, 300), (128, 2, 40, 600), (96, 4, 5, 70)):
+        p = pool_with(hd + 2, n, hd)
+        p.scale[:, :, :, :, 1] *= np.float32(size)
+        q = np.random.default_rng(n).normal(0, 1, (rows, heads * hd)).astype(np.float32)
+        check(R.DevPool(dev, p), p, [0], [rows], q, heads, max_len=n)
