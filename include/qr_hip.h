@@ -415,7 +415,7 @@ int qr_decoder_prefill(qr_decoder* dec, const int32_t* tokens, int n, int pos0, 
 /* Pages of 8-bit K and V that several sequences share: batches, beams, the
  * continuations of one prompt, speculative verification.  No counterpart in
  * the reference, whose cache holds one sequence; the calls below promise the
- * formulas they state in fp32 accuracy, not another build's bits.
+ * formulas they state to the accuracy they state, not another build's bits.
  *
  * All memory is the caller's, on the context's device:
  *   data   int8 [n_layers][n_pages][n_kv_heads][page / 16][2][16 * head_dim],
@@ -439,8 +439,8 @@ int qr_decoder_prefill(qr_decoder* dec, const int32_t* tokens, int n, int pos0, 
  * QR_KV_MAX_LIST.  What a list asks for is checked on the device: `status`
  * (device int32, optional) receives QR_OK; QR_ERR_INVALID for a sequence that
  * does not exist, one listed twice (extend, and dst of assign), a negative
- * number, or more tokens than max_pages hold; QR_ERR_NOMEM where the free pages do not
- * suffice.  A call whose status is not QR_OK has changed nothing. */
+ * number, more tokens than max_pages hold, or (extend) a partly filled page that the table
+ * lacks; QR_ERR_NOMEM where the free pages do not suffice.  A call whose status is not QR_OK has changed nothing. */
 #define QR_KV_BLOCK 16
 #define QR_KV_MAX_LIST 4096
 #define QR_KV_MAX_SEQS 65536
@@ -498,12 +498,14 @@ int qr_kv_pool_compact(qr_ctx* ctx, const qr_kv_pool* pool, int32_t* map, int32_
  * store quantizes K and V rows (fp32, head h's values at h * head_dim, row
  * stride kv_stride, a multiple of 4, 16-byte aligned) into layer `layer`.  A block's scale becomes
  * max(its scale if it holds older tokens, max |x| / 127) over the new finite
- * values; new values are x / scale rounded to the nearest even integer, and
- * where the scale grew older ones are rounded to the new one.  NaN is stored as 0,
- * an infinity as +-127.  A row before position 0, or where the table has no
- * page, is not stored.  No sequence may be listed twice, and none of the pages
+ * values; new values are x / scale rounded to the nearest integer (ties to even), at most
+ * 127 either way, and where the scale grew older ones are rounded to the new one.  NaN is stored
+ * as 0, an infinity as +-127, all of a block whose scale is 0 as 0 (one of nothing but zeros,
+ * NaN and infinities).  A scale does not fall while its block holds older tokens: where a trim
+ * drops those that raised it, as rejected drafts may, the older ones stay rounded to the larger
+ * scale.  A row before position 0, or where the table has no page, is not stored.  No sequence may be listed twice, and none of the pages
  * written shared: extend sees to that.
- * load reads rows back as fp32 (zeros for a row before position 0 or without a page). */
+ * load reads rows back as fp32 (+0 for a row before position 0 or without a page). */
 int qr_kv_pool_store(qr_ctx* ctx, const qr_kv_pool* pool, int layer, const int32_t* seqs,
                      const int32_t* start, int n, int T, const float* k, const float* v,
                      long kv_stride);
@@ -518,8 +520,13 @@ int qr_kv_pool_load(qr_ctx* ctx, const qr_kv_pool* pool, int layer, const int32_
  * aligned.  scale <= 0 means 1 / sqrtf(head_dim).  max_len bounds the
  * sequences' lengths for the split of the work (0: max_pages * page); longer
  * sequences are served all the same.  A row that sees no token (one before
- * position 0) gives zeros, a q row that is not finite NaN.  A sequence may be listed more than
- * once; out must not overlap q. */
+ * position 0) gives zeros; of others, a head whose q is not finite gives NaN.  A sequence may be
+ * listed more than once; out must not overlap q.
+ *
+ * Accuracy: sums are fp32 over exact products, softmax statistics fp32.  A value of q is held
+ * to 2^-22 of itself or 2^-50 of the largest of its head's row, whichever is more, a weight
+ * times its block's V scale to 2^-22 of itself or 2^-50 of the row's largest; a score rounds
+ * as an fp32 number does, and with it its token's weight. */
 int qr_kv_pool_attention(qr_ctx* ctx, const qr_kv_pool* pool, int layer, const int32_t* seqs,
                          const int32_t* start, int n, int T, int n_heads, const float* q,
                          long q_stride, float* out, long out_stride, int max_len, int window,

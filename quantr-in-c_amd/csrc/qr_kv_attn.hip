@@ -6,8 +6,7 @@
 //   s_t = scale q . k_t,  out = sum_t exp(s_t) v_t / sum_t exp(s_t).
 // The other operand of each product is an fp32 number, a row's q or a token's weight: two fp16
 // pieces, the nearest one and 2048 times what it leaves, hold it to 2^-22 of itself (a
-// score's own roundings in fp32 move a weight more) or 2^-50 of the largest of its row (q) or of 256
-// tokens (weights).  The cache's bytes are widened to fp16 on the way, 1.25 instructions
+// score's own roundings in fp32 move a weight more) or 2^-50 of the largest of its row.  The cache's bytes are widened to fp16 on the way, 1.25 instructions
 // each; products are exact and sums fp32, each piece's apart.  (Digits of the largest on int8
 // products, 40 us for a prompt's 512 rows where this takes 48, gave the small ones up: beside a token
 // that takes 0.9999 of the weight with values of 0 the output was off by a fifth of itself,
