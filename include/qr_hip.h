@@ -466,7 +466,8 @@ int qr_kv_pool_reset(qr_ctx* ctx, const qr_kv_pool* pool);
 /* Sequence seqs[i] grows by add[i] tokens: it takes the pages that they need,
  * the free pages in ascending order in the order of the list.  Where its last
  * page is partly filled and shared, it first takes a copy of it (of all
- * layers): in the order of the list, each of them as long as another sequence holds it. */
+ * layers): in the order of the list, each of them as long as another sequence
+ * holds it. */
 int qr_kv_pool_extend(qr_ctx* ctx, const qr_kv_pool* pool, const int32_t* seqs,
                       const int32_t* add, int n, int32_t* status);
 
@@ -488,12 +489,14 @@ int qr_kv_pool_trim(qr_ctx* ctx, const qr_kv_pool* pool, const int32_t* seqs,
  * [n_pages], optional) each page's new number, -1 for a free page. */
 int qr_kv_pool_compact(qr_ctx* ctx, const qr_kv_pool* pool, int32_t* map, int32_t* n_live);
 
-/* The rows of a ragged batch: T rows (at most QR_KV_MAX_ROWS), of which start[i] .. start[i + 1] - 1
- * (start: device int32 [n + 1], ascending) are sequence seqs[i]'s (seqs null:
- * sequence i's), n up to QR_KV_MAX_SEQS; they stand for its last positions, so a call that brings new
- * tokens extends first.  Rows that no sequence owns are left as they are.  A sequence that
- * does not exist counts as empty.  `start` is not checked: entries outside 0 .. T are cut to it, and
- * where they do not ascend results are undefined, but only rows below T are read or written.
+/* The rows of a ragged batch: T rows (at most QR_KV_MAX_ROWS), of which start[i]
+ * .. start[i + 1] - 1 (start: device int32 [n + 1], ascending) are sequence
+ * seqs[i]'s (seqs null: sequence i's), n up to QR_KV_MAX_SEQS; they stand for its
+ * last positions, so a call that brings new tokens extends first.  Rows that no
+ * sequence owns are left as they are.  A sequence that does not exist counts as
+ * empty.  `start` is not checked: entries outside 0 .. T are cut to it, and where
+ * they do not ascend results are undefined, but only rows below T are read or
+ * written.
  *
  * store quantizes K and V rows (fp32, head h's values at h * head_dim, row
  * stride kv_stride, a multiple of 4, 16-byte aligned) into layer `layer`.  A block's scale becomes
@@ -537,15 +540,15 @@ int qr_kv_pool_attention(qr_ctx* ctx, const qr_kv_pool* pool, int layer, const i
 /* For each of `rows` rows of `vocab` logits (row stride `stride`), with p =
  * softmax(row): lp[r] = log p[targets[r]]; entropy[r] = -sum p log p; rank[r]
  * = the number of logits ahead of the target's (greater ones, and equal ones
- * of lower index); top_id / top_lp [r][n_top], n_top <= QR_LOGPROBS_MAX_TOP: the most
- * probable tokens, equal ones by ascending index, with their log
- * probabilities (id -1 and -inf behind the vocabulary).  rows <= 2^23, vocab <= 2^30.  Each output may be
- * null; targets may be null where lp and rank are.  A target outside the
- * vocabulary gives lp 0 and rank -1.  Logits of -inf have probability 0; a row
- * of nothing else gives lp -inf, entropy 0.  A row that holds a NaN or +inf
- * gives NaN for lp, entropy and top_lp; in its order a NaN counts as -inf.  Beside
- * qr_decoder_prefill with QR_PREFILL_ALL_LOGITS it scores a prompt; no
- * counterpart in the reference. */
+ * of lower index); top_id / top_lp [r][n_top], n_top <= QR_LOGPROBS_MAX_TOP: the
+ * most probable tokens, equal ones by ascending index, with their log
+ * probabilities (id -1 and -inf behind the vocabulary).  rows <= 2^23, vocab <=
+ * 2^30.  Each output may be null; targets may be null where lp and rank are.  A
+ * target outside the vocabulary gives lp 0 and rank -1.  Logits of -inf have
+ * probability 0; a row of nothing else gives lp -inf, entropy 0.  A row that holds
+ * a NaN or +inf gives NaN for lp, entropy and top_lp; in its order a NaN counts as
+ * -inf.  Beside qr_decoder_prefill with QR_PREFILL_ALL_LOGITS it scores a prompt;
+ * no counterpart in the reference. */
 #define QR_LOGPROBS_MAX_TOP 64
 int qr_logprobs(qr_ctx* ctx, const float* logits, long stride, int rows, int vocab,
                 const int32_t* targets, float* lp, float* entropy, int32_t* rank, int n_top,

@@ -5,13 +5,14 @@
 // values, one scale per block b of 16 tokens):
 //   s_t = scale q . k_t,  out = sum_t exp(s_t) v_t / sum_t exp(s_t).
 // The other operand of each product is an fp32 number, a row's q or a token's weight: two fp16
-// pieces, the nearest one and 2048 times what it leaves, hold it to 2^-22 of itself (a
-// score's own roundings in fp32 move a weight more) or 2^-50 of the largest of its row.  The cache's bytes are widened to fp16 on the way, 1.25 instructions
-// each; products are exact and sums fp32, each piece's apart.  (Digits of the largest on int8
-// products, 40 us for a prompt's 512 rows where this takes 48, gave the small ones up: beside a token
-// that takes 0.9999 of the weight with values of 0 the output was off by a fifth of itself,
-// beside a channel of q of 10^6 by a fortieth.  Three bf16 pieces of the weights, which know no
-// largest, took 50 us where two of fp16 took 44.)
+// pieces, the nearest one and 2048 times what it leaves, hold it to 2^-22 of itself (a score's
+// own roundings in fp32 move a weight more) or 2^-50 of the largest of its row.  The cache's
+// bytes are widened to fp16 on the way, 1.25 instructions each; products are exact and sums
+// fp32, each piece's apart.  (Digits of the largest on int8 products, 40 us for a prompt's 512
+// rows where this takes 48, gave the small ones up: beside a token that takes 0.9999 of the
+// weight with values of 0 the output was off by a fifth of itself, beside a channel of q of 10^6
+// by a fortieth.  Three bf16 pieces of the weights, which know no largest, took 50 us where
+// two of fp16 took 44.)
 //
 // A workgroup of four waves serves a tile of 16 or 32 rows (queries times the query
 // heads of a kv head) and takes 256 tokens a round, a wave 64 of them.  A wave's four
@@ -27,11 +28,12 @@
 // pieces from LDS (16 KiB).  A wave that kept all columns of its own tokens instead converted four
 // times as many sums, held 206 registers for 164, and ended in a join of the waves.
 //
-// What bounds it: many rows, the issue of VALU instructions beside the matrix ones (a
-// prompt's 512 rows of 8 heads a kv head at 1501 .. 2012: 42 us, VALU busy for 23 of them, MFMA
-// 9); a wave in its products goes before the other wave of its SIMD, so that one's products run
-// under the other's softmax (46 us without it).  One row a sequence, two launches' latency and
-// then HBM (32 of 512 .. 4096 tokens, 54 MB: 21 us; one of 702: 8.0).
+// What bounds it.  Many rows: neither unit alone (a prompt's 512 rows of 8 heads a kv head at
+// 1501 .. 2012, 47 us: VALU issue 52 % of the time, matrix units 23 %); of a wave's time 30 % goes
+// by waiting to issue beside the SIMD's other wave and 27 % at barriers and for memory.  A wave
+// in its products goes before the other one, so that one's products run under the other's softmax
+// (52 us without it).  One row a sequence: two launches' latency, the widening, and then HBM (32 of
+// 587 .. 4096 tokens, 66 MB: 23.5 us; one of 702: 9.1).
 //
 // The weights carry V's scale: with vs = f 2^e (1/2 <= f < 1), w_t = f 2^(s_t
 // log2(e) + e - M) against a reference M that brings the round's largest weight just
@@ -410,7 +412,8 @@ __global__ __launch_bounds__(256, HD <= 128 && RT == 1 ? 3 : 2) void k_pool_attn
           for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int i = 0; i < 2; i++)
-              qd[r][k][h][i] = *reinterpret_cast<const v8h*>(&sq[i][16 * r + n][64 * k + 16 * g + 8 * h]);
+              qd[r][k][h][i] =
+                  *reinterpret_cast<const v8h*>(&sq[i][16 * r + n][64 * k + 16 * g + 8 * h]);
 #pragma unroll
       for (int tt = 0; tt < 4; tt++) {
         v4f acc[RT][2];
@@ -733,10 +736,10 @@ __global__ __launch_bounds__(256) void k_pool_attn_join(AttnArgs a) {
 // one with the least time by what was measured (us): 4.5 before a workgroup's first
 // round and after its last, 0.7 + 0.014 head_dim a round, 5 for a thousand workgroups, 4 for
 // joining parts; 768 workgroups at once (512 where registers allow two a CU), of
-// several sequences 0.6 of the longest's parts filled.  (702 tokens of head_dim 64: one part 9.2,
-// three 9.6; 1500 of 128: one 19.7, six 11.3; 16 sequences of up to 1024: one 15.0, four 12.1; 64 of them:
-// one 17.2, four 19.3; 32 of up to 4096: eight 23.8, four 24.3, sixteen 27.9; 8 of up to 2000 of
-// head_dim 256: eight 14.2, four 18.5.)
+// several sequences 0.6 of the longest's parts filled.  (702 tokens of head_dim 64: one part
+// 9.2, three 9.6; 1500 of 128: one 19.7, six 11.3; 16 sequences of up to 1024: one 15.0, four
+// 12.1; 64 of them: one 17.2, four 19.3; 32 of up to 4096: eight 23.8, four 24.3, sixteen 27.9;
+// 8 of up to 2000 of head_dim 256: eight 14.2, four 18.5.)
 AttnArgs attn_plan(const PoolView& p, const Ragged& r, int n_heads, int max_len, int window) {
   AttnArgs a = {};
   a.p = p;
