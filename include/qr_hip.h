@@ -439,8 +439,9 @@ int qr_decoder_prefill(qr_decoder* dec, const int32_t* tokens, int n, int pos0, 
  * QR_KV_MAX_LIST.  What a list asks for is checked on the device: `status`
  * (device int32, optional) receives QR_OK; QR_ERR_INVALID for a sequence that
  * does not exist, one listed twice (extend, and dst of assign), a negative
- * number, more tokens than max_pages hold, or (extend) a partly filled page that the table
- * lacks; QR_ERR_NOMEM where the free pages do not suffice.  A call whose status is not QR_OK has changed nothing. */
+ * number, more tokens than max_pages hold, or (extend) a partly filled page that
+ * the table lacks; QR_ERR_NOMEM where the free pages do not suffice.  A call whose
+ * status is not QR_OK has changed nothing. */
 #define QR_KV_BLOCK 16
 #define QR_KV_MAX_LIST 4096
 #define QR_KV_MAX_SEQS 65536
@@ -498,16 +499,17 @@ int qr_kv_pool_compact(qr_ctx* ctx, const qr_kv_pool* pool, int32_t* map, int32_
  * they do not ascend results are undefined, but only rows below T are read or
  * written.
  *
- * store quantizes K and V rows (fp32, head h's values at h * head_dim, row
- * stride kv_stride, a multiple of 4, 16-byte aligned) into layer `layer`.  A block's scale becomes
- * max(its scale if it holds older tokens, max |x| / 127) over the new finite
- * values; new values are x / scale rounded to the nearest integer (ties to even), at most
- * 127 either way, and where the scale grew older ones are rounded to the new one.  NaN is stored
- * as 0, an infinity as +-127, all of a block whose scale is 0 as 0 (one of nothing but zeros,
- * NaN and infinities).  A scale does not fall while its block holds older tokens: where a trim
- * drops those that raised it, as rejected drafts may, the older ones stay rounded to the larger
- * scale.  A row before position 0, or where the table has no page, is not stored.  No sequence may be listed twice, and none of the pages
- * written shared: extend sees to that.
+ * store quantizes K and V rows (fp32, head h's values at h * head_dim, row stride
+ * kv_stride, a multiple of 4, 16-byte aligned) into layer `layer`.  A block's
+ * scale becomes max(its scale if it holds older tokens, max |x| / 127) over the
+ * new finite values; new values are x / scale rounded to the nearest integer (ties
+ * to even), at most 127 either way, and where the scale grew older ones are rounded
+ * to the new one.  NaN is stored as 0, an infinity as +-127, all of a block whose
+ * scale is 0 as 0 (one of nothing but zeros, NaN and infinities).  A scale does not
+ * fall while its block holds older tokens: where a trim drops those that raised it,
+ * as rejected drafts may, the older ones stay rounded to the larger scale.  A row
+ * before position 0, or where the table has no page, is not stored.  No sequence
+ * may be listed twice, and none of the pages written shared: extend sees to that.
  * load reads rows back as fp32 (+0 for a row before position 0 or without a page). */
 int qr_kv_pool_store(qr_ctx* ctx, const qr_kv_pool* pool, int layer, const int32_t* seqs,
                      const int32_t* start, int n, int T, const float* k, const float* v,
