@@ -528,10 +528,11 @@ int qr_kv_pool_load(qr_ctx* ctx, const qr_kv_pool* pool, int layer, const int32_
  * position 0) gives zeros; of others, a head whose q is not finite gives NaN.  A sequence may be
  * listed more than once; out must not overlap q.
  *
- * Accuracy: sums are fp32 over exact products, softmax statistics fp32.  A value of q is held
- * to 2^-22 of itself or 2^-50 of the largest of its head's row, whichever is more, a weight
- * times its block's V scale to 2^-22 of itself or 2^-50 of the row's largest; a score rounds
- * as an fp32 number does, and with it its token's weight. */
+ * Accuracy: sums are fp32 over exact products, softmax statistics fp32.  A value of
+ * q is held to 2^-22 of itself or 2^-50 of the largest of its head's row (2^-147
+ * where that is less), whichever is more, a weight times its block's V scale to
+ * 2^-22 of itself or 2^-50 of the row's largest; a score rounds as an fp32 number
+ * does, and with it its token's weight. */
 int qr_kv_pool_attention(qr_ctx* ctx, const qr_kv_pool* pool, int layer, const int32_t* seqs,
                          const int32_t* start, int n, int T, int n_heads, const float* q,
                          long q_stride, float* out, long out_stride, int max_len, int window,

@@ -3,8 +3,8 @@
 //
 // A block is 16 tokens of one kv head of one layer: int8 K [16][hd], then int8
 // V [hd][16], and two fp32 scales.  V lies column by column, so that 16 bytes
-// of it are one column's 16 tokens: what a lane of a 16x16x64 int8 MFMA takes
-// as its operand of the value product.
+// of it are one column's 16 tokens: what a lane widens to its operands of two
+// 16x16x32 fp16 MFMA of the value product.
 #pragma once
 
 #include <hip/hip_runtime.h>
