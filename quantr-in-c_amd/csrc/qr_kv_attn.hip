@@ -9,7 +9,7 @@
 // own roundings in fp32 move a weight more) or 2^-50 of the largest of its row.  The cache's
 // bytes are widened to fp16 on the way, 1.25 instructions each; products are exact and sums
 // fp32, each piece's apart.  (Digits of the largest on int8 products, 40 us for a prompt's 512
-// rows where this takes 48, gave the small ones up: beside a token that takes 0.9999 of the
+// rows where this takes 47, gave the small ones up: beside a token that takes 0.9999 of the
 // weight with values of 0 the output was off by a fifth of itself, beside a channel of q of 10^6
 // by a fortieth.  Three bf16 pieces of the weights, which know no largest, took 50 us where
 // two of fp16 took 44.)
